@@ -1,4 +1,5 @@
-"""ctypes binding of libsbamd.so (the C ABI declared in include/sbamd_gemm.h and include/sbamd_dist.h).
+"""ctypes binding of libsbamd.so (the C ABI declared in include/sbamd_gemm.h, include/sbamd_dist.h and
+include/sbamd_ffn.h).
 
 The library is loaded from the source tree (sycl_blas_amd/lib/libsbamd.so, built
 by sycl_blas_amd/csrc/Makefile).  There is no fallback: if the shared object is
@@ -124,6 +125,20 @@ for _p, _sc in (("s", _f32), ("d", _f64)):
     DIST_SIGNATURES[f"sbamd_dist_gathered_{_p}gemm"] = (_int, _dist_gemm_sig(_sc) + [_int, _int])
     DIST_SIGNATURES[f"sbamd_dist_splitk_{_p}gemm"] = (_int, _dist_gemm_sig(_sc) + [_int, _int])
 
+# ---- the feed-forward layers (include/sbamd_ffn.h)
+ACT_SILU, ACT_GELU, ACT_GELU_TANH, ACT_RELU = 0, 1, 2, 3
+I8_MAX_K = 131071
+
+FFN_SIGNATURES = {}
+for _p in "shb":
+    FFN_SIGNATURES[f"sbamd_{_p}quantize_i8"] = (_int, [_vp, _i64, _i64, _vp, _i64, _vp, _i64, _vp])
+    FFN_SIGNATURES[f"sbamd_i8{_p}gemm"] = (_int, [_vp, _ch, _ch, _i64, _i64, _i64, _f32, _vp, _i64, _vp, _vp, _i64, _vp, _f32, _vp, _i64])
+    FFN_SIGNATURES[f"sbamd_i8{_p}gated_gemm"] = (_int, [_vp, _int, _ch, _ch, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64])
+for _p in "hb":
+    FFN_SIGNATURES[f"sbamd_{_p}gated_gemm"] = (_int, [_vp, _int, _ch, _ch, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64])
+    FFN_SIGNATURES[f"sbamd_{_p}gated_gemm_grad"] = (_int, [_vp, _int, _ch, _ch, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp,
+                                                           _i64, _vp, _i64, _f32, _vp, _i64, _f32, _vp, _i64])
+
 _lib = None
 
 
@@ -138,7 +153,7 @@ def load():
             "(or `python -c 'import __graft_entry__ as g; g.build()'`). "
             "There is no CPU fallback for the GEMM path.")
     lib = C.CDLL(LIB_PATH)
-    for name, (res, args) in list(SIGNATURES.items()) + list(DIST_SIGNATURES.items()):
+    for name, (res, args) in list(SIGNATURES.items()) + list(DIST_SIGNATURES.items()) + list(FFN_SIGNATURES.items()):
         fn = getattr(lib, name)  # AttributeError if the ABI lost a symbol
         fn.restype = res
         fn.argtypes = args

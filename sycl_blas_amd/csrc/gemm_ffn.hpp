@@ -1,0 +1,535 @@
+// Kernels of the feed-forward entry points (include/sbamd_ffn.h): products of 8-bit
+// integers with scales, the gated block in 16 and 8 bits, token quantisation and the
+// elementwise half of the gated block's gradient.
+//
+// Layout: the column-major C is m (channels, contiguous) x n (tokens).  Both operands are
+// read along k ([channel][k] and [token][k]); the host repacks what lies otherwise.
+// Lengths along k are in BYTES throughout, so one kernel serves 16-bit and 8-bit
+// operands: a matrix-instruction fragment is 16 bytes per lane for either (8 k of a
+// 16-bit type, 16 k of an 8-bit one), and the order in which k is walked does not matter
+// as long as both operands share it.
+#pragma once
+
+#include "gemm_half.hpp"
+#include "../../include/sbamd_ffn.h"
+
+namespace sbamd {
+
+struct I8Tag {};  // 8-bit integers, 32-bit integer sums
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+// 16 bytes at any address (global memory takes a misaligned vector; the type says so to the compiler)
+typedef u16x8 u16x8_at1 __attribute__((aligned(1)));
+
+// 16 x 16 matrix instruction: op0 carries the token index, op1 the channel; lane l ends up with channel l % 16 and
+// tokens 4 * (l / 16) .. + 3.  K: 32 of a 16-bit type, 64 of 8-bit integers.
+template <typename Tag>
+struct FfnMma;
+template <>
+struct FfnMma<HalfTag> {
+  static constexpr int BYTES = 2;
+  using acc_t = f32x4_t;
+  using sum_t = float;
+  __device__ static inline acc_t mma(u16x8 x, u16x8 y, acc_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), c, 0, 0, 0);
+  }
+};
+template <>
+struct FfnMma<Bf16Tag> {
+  static constexpr int BYTES = 2;
+  using acc_t = f32x4_t;
+  using sum_t = float;
+  __device__ static inline acc_t mma(u16x8 x, u16x8 y, acc_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
+  }
+};
+template <>
+struct FfnMma<I8Tag> {
+  static constexpr int BYTES = 1;
+  using acc_t = i32x4;
+  using sum_t = int;
+  __device__ static inline acc_t mma(u16x8 x, u16x8 y, acc_t c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, x), __builtin_bit_cast(i32x4, y), c, 0, 0, 0);
+  }
+};
+
+template <typename TOut>
+struct FfnArgs {
+  const unsigned char* a;  // [rows][k bytes], rows = m or 2m
+  const unsigned char* b;  // [n][k bytes]
+  int64_t lda, ldb;        // bytes from one row to the next
+  int64_t m, n, kb;        // channels of C, tokens, bytes along k
+  const float* scale_a;    // per row of a, NULL = ones
+  const float* scale_b;    // per token, NULL = ones
+  TOut* c;
+  int64_t ldc;
+  TOut* p;                 // pre-activations (2m x n) or NULL; gated only
+  int64_t ldp;
+  float alpha, beta;
+  int32_t beta_zero;
+  int32_t act;
+  int32_t tiles_m, tiles_n;
+};
+
+// ---------------------------------------------------------------- activations
+// e^x through the hardware's 2^x (1 ulp): the argument's rounding makes it good to about |x| * 2^-24, far below
+// the 16-bit roundings behind it and within 4e-6 for a float result.  Overflow gives infinity and a quotient of 0.
+__device__ inline float ffn_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
+__device__ inline float ffn_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + ffn_exp(-x)); }
+
+// tanh(y) = 2 sigmoid(2y) - 1, so 0.5 g (1 + tanh(y)) = g sigmoid(2y), without the cancellation for negative g.
+__device__ inline float gelu_tanh_arg2(float g) { return 1.5957691216057308f * (g + 0.044715f * g * g * g); }
+
+__device__ inline float act_value(int act, float g) {
+  switch (act) {
+    case SBAMD_ACT_SILU: return g * ffn_sigmoid(g);
+    case SBAMD_ACT_GELU: return 0.5f * g * erfcf(-0.70710678118654752f * g);  // 2 Phi(g) = erfc(-g / sqrt(2))
+    case SBAMD_ACT_GELU_TANH: return g * ffn_sigmoid(gelu_tanh_arg2(g));
+    default: return g <= 0.0f ? 0.0f : g;  // NaN stays NaN
+  }
+}
+
+// act(g) and act'(g)
+__device__ inline void act_value_slope(int act, float g, float& value, float& slope) {
+  switch (act) {
+    case SBAMD_ACT_SILU: {
+      const float s = ffn_sigmoid(g);
+      value = g * s;
+      slope = s + value * (1.0f - s);
+      break;
+    }
+    case SBAMD_ACT_GELU: {
+      const float phi = 0.5f * erfcf(-0.70710678118654752f * g);
+      value = g * phi;
+      slope = phi + g * 0.3989422804014327f * ffn_exp(-0.5f * g * g);
+      break;
+    }
+    case SBAMD_ACT_GELU_TANH: {
+      // value = g s(z), z = 2 sqrt(2/pi) (g + 0.044715 g^3); slope = s + g s (1 - s) z'.  Far out s (1 - s) is 0
+      // and z' is not: the product is taken only where s (1 - s) is not 0 (0 * inf would be NaN).
+      const float s = ffn_sigmoid(gelu_tanh_arg2(g));
+      value = g * s;
+      const float bell = s * (1.0f - s);
+      slope = bell > 0.0f ? s + g * bell * (1.5957691216057308f * (1.0f + 0.134145f * g * g)) : s;
+      break;
+    }
+    default:
+      value = g <= 0.0f ? 0.0f : g;
+      slope = g > 0.0f ? 1.0f : (g == g ? 0.0f : g);
+  }
+}
+
+// One integer or float sum -> the scaled float: ((sum * sa) * sb), in this order so that two tiny scales do not
+// underflow against each other.
+template <typename Sum>
+__device__ inline float ffn_scaled(Sum s, float sa, float sb) {
+  return (float(s) * sa) * sb;
+}
+
+// ------------------------------------------------------------- narrow kernel
+// C for a block of 32 operand rows (32 channels, or 16 gates with their 16 partners) and 16 * NB tokens.  The W
+// wavefronts of the workgroup share out k in chunks of 128 bytes (chunk c goes to wavefront c % W: together they walk W
+// whole cache lines of each row at a time) and join their sums through LDS in wavefront order, so few rows still put many
+// loads in flight and no second launch and no workspace is needed.  A wavefront's chunk goes global -> registers
+// (lane = one 16-byte piece, 8 lanes = one row's cache line; DEPTH chunks ahead) -> its own corner of LDS -> fragments:
+// the detour through LDS turns the coalesced pieces into the matrix instruction's layout.  No barrier inside the loop:
+// LDS operations of one wavefront execute in order.  Bound by the weights' way out of memory for few tokens.
+constexpr int NARROW_CHUNK = 128, NARROW_WAVES = 4, NARROW_ROWS = 32;
+
+// Image: 128-byte rows of eight 16-byte pieces; piece c of row r sits at c ^ ((r >> 1) & 7).  A fragment read has 16 lanes
+// on 16 rows at the same c: two rows share a turn of the 64 banks, the eight pairs are told apart by the XOR.
+__device__ inline int narrow_slot(int row, int piece) { return row * NARROW_CHUNK + ((piece ^ ((row >> 1) & 7)) << 4); }
+
+template <int NB>
+constexpr int narrow_lds_bytes() {
+  constexpr int stage = NARROW_WAVES * (NARROW_ROWS + 16 * NB) * NARROW_CHUNK;
+  constexpr int join = NARROW_WAVES * 16 * NB * (NARROW_ROWS + 1) * 4;
+  return stage > join ? stage : join;
+}
+
+template <typename Tag, typename TOut, bool GATED, int NB, int DEPTH>
+__global__ void __launch_bounds__(NARROW_WAVES * 64) ffn_narrow_kernel(const FfnArgs<TOut> g) {
+  using M = FfnMma<Tag>;
+  using Sum = typename M::sum_t;
+  constexpr int W = NARROW_WAVES, ROWS = NARROW_ROWS, TOK = 16 * NB;
+  constexpr int CH = GATED ? ROWS / 2 : ROWS;  // channels of C per workgroup
+  constexpr int LA = ROWS / 8, LB = TOK / 8, NL = LA + LB;  // load instructions per chunk
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
+  SBAMD_LDS unsigned char* smem = (SBAMD_LDS unsigned char*)smem_raw;
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int logical = xcd_remap(blockIdx.x, gridDim.x);
+  const int tm = logical / g.tiles_n, tn = logical - tm * g.tiles_n;  // the token blocks of one row block are neighbours
+  const int64_t m0 = int64_t(tm) * CH, n0 = int64_t(tn) * TOK;
+
+  // Rows past the edge read the last valid one: they only feed elements that are never stored.
+  const int piece = lane & 7, row8 = lane >> 3;
+  const unsigned char* src[NL];
+#pragma unroll
+  for (int i = 0; i < NL; ++i) {
+    if (i < LA) {
+      const int row = i * 8 + row8;
+      int64_t ch = m0 + (GATED ? row & 15 : row);
+      ch = ch < g.m ? ch : g.m - 1;
+      if (GATED && row >= 16) ch += g.m;
+      src[i] = g.a + ch * g.lda + piece * 16;
+    } else {
+      int64_t t = n0 + (i - LA) * 8 + row8;
+      t = t < g.n ? t : g.n - 1;
+      src[i] = g.b + t * g.ldb + piece * 16;
+    }
+  }
+
+  typename M::acc_t acc[2][NB];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[i][j][r] = 0;
+
+  SBAMD_LDS unsigned char* mine = smem + wave * (ROWS + TOK) * NARROW_CHUNK;
+  u16x8 reg[DEPTH][NL];
+  auto issue = [&](u16x8 (&v)[NL], int64_t chunk) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) v[i] = *reinterpret_cast<const u16x8_at1*>(src[i] + chunk * NARROW_CHUNK);
+  };
+  auto consume = [&](const u16x8 (&v)[NL]) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int row = i < LA ? i * 8 + row8 : (i - LA) * 8 + row8;
+      *reinterpret_cast<SBAMD_LDS u16x8*>(mine + (i < LA ? 0 : ROWS * NARROW_CHUNK) + narrow_slot(row, piece)) = v[i];
+    }
+    // other lanes of this wavefront read what this lane wrote: keep the compiler from moving the reads up (the
+    // hardware keeps a wavefront's LDS operations in order)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      u16x8 fa[2], fb[NB];
+      const int at = 4 * s + (lane >> 4);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        fa[i] = *reinterpret_cast<const SBAMD_LDS u16x8*>(mine + narrow_slot(i * 16 + (lane & 15), at));
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+        fb[j] = *reinterpret_cast<const SBAMD_LDS u16x8*>(mine + ROWS * NARROW_CHUNK + narrow_slot(j * 16 + (lane & 15), at));
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[i][j] = M::mma(fb[j], fa[i], acc[i][j]);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  };
+
+  const int64_t whole = g.kb / NARROW_CHUNK;  // whole chunks; chunk wave + W * i is this wavefront's i-th
+  const int64_t count = whole > wave ? (whole - wave + W - 1) / W : 0;
+  const int64_t piped = count / DEPTH * DEPTH;
+  // the pipelined part: no branch between a load and its use, so the compiler's waits stay counted
+  if (piped > 0) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) issue(reg[d], wave + int64_t(W) * d);
+    for (int64_t it = DEPTH; it < piped; it += DEPTH) {
+#pragma unroll
+      for (int d = 0; d < DEPTH; ++d) {
+        consume(reg[d]);
+        issue(reg[d], wave + W * (it + d));
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) consume(reg[d]);
+  }
+  if (piped < count) {
+#pragma unroll
+    for (int d = 0; d < DEPTH - 1; ++d)
+      if (piped + d < count) issue(reg[d], wave + W * (piped + d));
+#pragma unroll
+    for (int d = 0; d < DEPTH - 1; ++d)
+      if (piped + d < count) consume(reg[d]);
+  }
+  // the last, partial chunk: zeros behind the end of k (the rows' ends are not read past)
+  const int rest = int(g.kb - whole * NARROW_CHUNK);
+  if (rest > 0 && wave == int(whole % W)) {
+    const int have = rest - piece * 16;  // bytes of this lane's piece that exist
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const unsigned char* s = src[i] + whole * NARROW_CHUNK;
+      u16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (have >= 16) {
+        v = *reinterpret_cast<const u16x8_at1*>(s);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          uint16_t x = 0;
+          if (2 * e < have) x = s[2 * e];
+          if (2 * e + 1 < have) x |= uint16_t(uint16_t(s[2 * e + 1]) << 8);
+          v[e] = x;
+        }
+      }
+      reg[0][i] = v;
+    }
+    consume(reg[0]);
+  }
+
+  // Join: [wavefront][token][row], rows padded to 33 words.
+  __syncthreads();
+  SBAMD_LDS Sum* part = (SBAMD_LDS Sum*)smem;
+  constexpr int LDJ = ROWS + 1;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        part[(wave * TOK + j * 16 + 4 * (lane >> 4) + r) * LDJ + i * 16 + (lane & 15)] = acc[i][j][r];
+  __syncthreads();
+  auto joined = [&](int tok, int row) {
+    Sum s = part[tok * LDJ + row];
+#pragma unroll
+    for (int w = 1; w < W; ++w) s = s + part[(w * TOK + tok) * LDJ + row];
+    return s;
+  };
+  for (int e = tid; e < CH * TOK; e += W * 64) {
+    const int ch = e % CH, tok = e / CH;
+    const int64_t mm = m0 + ch, nn = n0 + tok;
+    if (mm >= g.m || nn >= g.n) continue;
+    const float sb = g.scale_b ? g.scale_b[nn] : 1.0f;
+    if constexpr (GATED) {
+      const float gate = ffn_scaled(joined(tok, ch), g.scale_a ? g.scale_a[mm] : 1.0f, sb);
+      const float up = ffn_scaled(joined(tok, 16 + ch), g.scale_a ? g.scale_a[g.m + mm] : 1.0f, sb);
+      if (g.p) {
+        store_out(g.p + mm + nn * g.ldp, gate);
+        store_out(g.p + g.m + mm + nn * g.ldp, up);
+      }
+      store_out(g.c + mm + nn * g.ldc, act_value(g.act, gate) * up);
+    } else {
+      TOut* at = g.c + mm + nn * g.ldc;
+      float out = g.alpha * ffn_scaled(joined(tok, ch), g.scale_a ? g.scale_a[mm] : 1.0f, sb);
+      if (!g.beta_zero) out = out + g.beta * load_out(at);
+      store_out(at, out);
+    }
+  }
+}
+
+// -------------------------------------------------------------------- repack
+// dst[r][0 .. row_bytes) = row r of the operand along k, zeros from `kb` bytes on.
+// ACROSS: element (r, k) of the source lies at r + k * ld (elements of BYTES bytes), transposed through a 64 x 64
+// LDS tile; else at k + r * ld (any alignment).  row_bytes is a multiple of 64.
+template <int BYTES, bool ACROSS>
+__global__ void __launch_bounds__(256)
+    ffn_pack_kernel(const unsigned char* __restrict__ src, int64_t ld, unsigned char* __restrict__ dst, int64_t row_bytes, int64_t rows,
+                    int64_t k) {
+  using E = typename std::conditional<BYTES == 2, uint16_t, uint8_t>::type;
+  if constexpr (!ACROSS) {
+    const int64_t per = row_bytes / 16, v = int64_t(blockIdx.x) * 256 + threadIdx.x;
+    if (v >= per * rows) return;
+    const int64_t r = v / per, at = (v - r * per) * 16, kb = k * BYTES;
+    const unsigned char* s = src + r * ld * BYTES + at;
+    u16x8 out = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (at + 16 <= kb) {
+      out = *reinterpret_cast<const u16x8_at1*>(s);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        uint16_t x = 0;
+        if (at + 2 * e < kb) x = s[2 * e];
+        if (at + 2 * e + 1 < kb) x |= uint16_t(uint16_t(s[2 * e + 1]) << 8);
+        out[e] = x;
+      }
+    }
+    *reinterpret_cast<u16x8*>(dst + r * row_bytes + at) = out;
+  } else {
+    __shared__ E tile[64][64 + 4 / BYTES];
+    const int64_t kt = (row_bytes / BYTES + 63) / 64;
+    const int64_t r0 = int64_t(blockIdx.x) / kt * 64, k0 = int64_t(blockIdx.x) % kt * 64;
+    const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+    const E* in = reinterpret_cast<const E*>(src);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int64_t kk = k0 + y + 4 * i, r = r0 + x;
+      tile[y + 4 * i][x] = kk < k && r < rows ? in[r + kk * ld] : E(0);
+    }
+    __syncthreads();
+    E* out = reinterpret_cast<E*>(dst);
+    const int64_t row_elems = row_bytes / BYTES;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int64_t r = r0 + y + 4 * i, kk = k0 + x;
+      if (r < rows && kk < row_elems) out[kk + r * row_elems] = tile[x][y + 4 * i];
+    }
+  }
+}
+
+// -------------------------------------------------------------- quantisation
+// Storage -> float, eight elements at any address.
+struct F32Tag {};
+template <typename Tag>
+struct QuantIn {
+  using type = uint16_t;
+  __device__ static inline void load8(const uint16_t* p, float (&v)[8]) {
+    const u16x8 x = *reinterpret_cast<const u16x8_at1*>(p);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = widen(Tag{}, x[e]);
+  }
+  __device__ static inline float load(const uint16_t* p) { return widen(Tag{}, *p); }
+};
+template <>
+struct QuantIn<F32Tag> {
+  using type = float;
+  typedef f32x4_t f32x4_at4 __attribute__((aligned(4)));
+  __device__ static inline void load8(const float* p, float (&v)[8]) {
+    const f32x4_t x = *reinterpret_cast<const f32x4_at4*>(p), y = *reinterpret_cast<const f32x4_at4*>(p + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = x[e], v[4 + e] = y[e];
+  }
+  __device__ static inline float load(const float* p) { return *p; }
+};
+
+// The integer nearest to 127 x / largest, ties to even, as of the real quotient.  x * (127 / largest) in float is off by
+// less than 127 * 2^-23 < 2^-16, so only a result within 2^-14 of a half can round to the wrong side; those few (and
+// everything where 127 / largest does not fit a float) are divided in double: 127 x is exact there, and a quotient that is
+// no tie differs from one by more than 2^-33, so the double's rounding cannot make or break a tie.
+__device__ inline int quant_round(float x, float inv, float largest, bool tiny) {
+  const float r = x * inv;
+  const float q = __builtin_rintf(r);
+  if (tiny || __builtin_fabsf(r - q) > 0.5f - 0x1p-14f) return int(__builtin_rint(127.0 * double(x) / double(largest)));
+  return int(q);
+}
+
+// A column on TPC consecutive threads (64 or 256 / 1024: a whole workgroup).  Each thread keeps HOLD vectors of eight elements in
+// registers between finding the maximum and rounding, so a column is read once; what a longer column has beyond is
+// read again.  Bound by memory: 2 (4) bytes in and 1 out per element.
+template <typename Tag, int TPC, int HOLD>
+__global__ void __launch_bounds__(TPC < 256 ? 256 : TPC)
+    ffn_quantize_kernel(int64_t m, int64_t n, const typename QuantIn<Tag>::type* __restrict__ x, int64_t ldx, int8_t* __restrict__ q,
+                        int64_t ldq, float* __restrict__ scale) {
+  using In = QuantIn<Tag>;
+  constexpr int COLS = TPC < 256 ? 256 / TPC : 1;
+  typedef uint32_t u32x2_at1 __attribute__((ext_vector_type(2), aligned(1)));
+  const int t = threadIdx.x % TPC;
+  const int64_t col = int64_t(blockIdx.x) * COLS + threadIdx.x / TPC;
+  const bool live = col < n;  // (whole wavefronts are live or not)
+  const typename In::type* src = x + (live ? col : n - 1) * ldx;
+  const int64_t vecs = m / 8;
+  float held[HOLD][8];
+  uint32_t top = 0;  // the maximum of |x| as bits: a NaN is above infinity, infinity above all else
+  auto look = [&](float v) {
+    const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+    top = b > top ? b : top;
+  };
+#pragma unroll
+  for (int i = 0; i < HOLD; ++i) {
+    const int64_t v = t + int64_t(i) * TPC;
+    if (v < vecs) {
+      In::load8(src + v * 8, held[i]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) held[i][e] = 0.0f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < HOLD; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) look(held[i][e]);
+  for (int64_t v = t + int64_t(HOLD) * TPC; v < vecs; v += TPC) {
+    float y[8];
+    In::load8(src + v * 8, y);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) look(y[e]);
+  }
+  const int64_t last = vecs * 8 + t;  // the odd elements behind the last vector: one per thread
+  const float odd = last < m ? In::load(src + last) : 0.0f;
+  look(odd);
+#pragma unroll
+  for (int s = 32; s; s >>= 1) {
+    const uint32_t o = __shfl_xor(top, s, 64);
+    top = o > top ? o : top;
+  }
+  if constexpr (TPC > 64) {
+    __shared__ uint32_t tops[TPC / 64];
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < TPC / 64; ++w) top = tops[w] > top ? tops[w] : top;
+  }
+  if (!live) return;
+  const float largest = __uint_as_float(top);
+  if (t == 0) scale[col] = largest / 127.0f;
+  const bool blank = top == 0 || top >= 0x7f800000u;  // nothing but zeros, or something not finite: all zeros
+  const bool tiny = largest < 1e-30f;                  // 127 / largest could overflow
+  const float inv = blank || tiny ? 0.0f : 127.0f / largest;
+  int8_t* dst = q + col * ldq;
+  auto store8 = [&](int64_t v, const float (&y)[8]) {
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int r = blank ? 0 : quant_round(y[e], inv, largest, tiny);
+      w[e / 4] |= uint32_t(uint8_t(int8_t(r))) << (8 * (e % 4));
+    }
+    u32x2_at1 out = {w[0], w[1]};
+    *reinterpret_cast<u32x2_at1*>(dst + v * 8) = out;
+  };
+#pragma unroll
+  for (int i = 0; i < HOLD; ++i) {
+    const int64_t v = t + int64_t(i) * TPC;
+    if (v < vecs) store8(v, held[i]);
+  }
+  for (int64_t v = t + int64_t(HOLD) * TPC; v < vecs; v += TPC) {
+    float y[8];
+    In::load8(src + v * 8, y);
+    store8(v, y);
+  }
+  if (last < m) dst[last] = int8_t(blank ? 0 : quant_round(odd, inv, largest, tiny));
+}
+
+// -------------------------------------------------- gradient, elementwise half
+// dG = dC U act'(G), dU = dC act(G): eight channels of one token per thread.  p and dp may be the same matrix: a thread
+// reads what it overwrites, and nothing else, before it writes.  (Hence no __restrict__ on them.)
+template <typename Tag, typename TOut>
+__global__ void __launch_bounds__(256)
+    ffn_gate_grad_kernel(int act, int64_t m, int64_t n, const uint16_t* p, int64_t ldp, const uint16_t* dc, int64_t lddc, uint16_t* dp,
+                         int64_t lddp) {
+  const int64_t per = (m + 7) / 8;
+  const int64_t v = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (v >= per * n) return;
+  const int64_t col = v / per, i = (v - col * per) * 8;
+  const uint16_t* pg = p + col * ldp + i;
+  const uint16_t* pd = dc + col * lddc + i;
+  uint16_t* out = dp + col * lddp + i;
+  auto one = [&](uint16_t gb, uint16_t ub, uint16_t db, uint16_t& dg, uint16_t& du) {
+    float value, slope;
+    act_value_slope(act, widen(Tag{}, gb), value, slope);
+    const float d = widen(Tag{}, db);
+    TOut og, ou;
+    store_out(&og, d * widen(Tag{}, ub) * slope);
+    store_out(&ou, d * value);
+    dg = __builtin_bit_cast(uint16_t, og);
+    du = __builtin_bit_cast(uint16_t, ou);
+  };
+  if (i + 8 <= m) {
+    const u16x8 gv = *reinterpret_cast<const u16x8_at1*>(pg), uv = *reinterpret_cast<const u16x8_at1*>(pg + m);
+    const u16x8 dv = *reinterpret_cast<const u16x8_at1*>(pd);
+    u16x8 og, ou;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      uint16_t x, y;
+      one(gv[e], uv[e], dv[e], x, y);
+      og[e] = x;
+      ou[e] = y;
+    }
+    *reinterpret_cast<u16x8_at1*>(out) = og;
+    *reinterpret_cast<u16x8_at1*>(out + m) = ou;
+  } else {
+    for (int e = 0; i + e < m; ++e) {
+      uint16_t x, y;
+      one(pg[e], pg[m + e], pd[e], x, y);
+      out[e] = x;
+      out[m + e] = y;
+    }
+  }
+}
+
+}  // namespace sbamd

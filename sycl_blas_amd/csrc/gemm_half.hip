@@ -1,4 +1,5 @@
-// 16-bit storage back end: half -> half, half -> float, bfloat16 -> float.
+// 16-bit storage back end: half -> half, half -> float, bfloat16 -> float, and bfloat16 -> bfloat16 for the
+// gradients of the gated block.
 #include <cmath>
 
 #include "gemm_dispatch.hpp"
@@ -398,6 +399,9 @@ hipError_t run_gemm_hs(Handle* h, const Problem<uint16_t, float>& p, float alpha
 }
 hipError_t run_gemm_bs(Handle* h, const Problem<uint16_t, float>& p, float alpha, float beta) {
   return run16<Bf16Tag, float>(h, p, alpha, beta);
+}
+hipError_t run_gemm_b(Handle* h, const Problem<uint16_t, bf16_bits>& p, float alpha, float beta) {
+  return run16<Bf16Tag, bf16_bits>(h, p, alpha, beta);
 }
 
 hipError_t run_scale_f16(Handle* h, uint16_t* c, int64_t rows, int64_t cols, int64_t ld, int64_t stride,

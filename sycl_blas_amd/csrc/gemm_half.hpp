@@ -57,7 +57,9 @@ struct Mfma16<Bf16Tag> {
 // Output conversion (one rounding, round-to-nearest-even; NaN stays NaN).
 __device__ inline float load_out(const float* p) { return *p; }
 __device__ inline float load_out(const uint16_t* p) { return float(__builtin_bit_cast(_Float16, *p)); }
+__device__ inline float load_out(const bf16_bits* p) { return __uint_as_float(uint32_t(p->v) << 16); }
 __device__ inline void store_out(float* p, float v) { *p = v; }
+__device__ inline void store_out(bf16_bits* p, float v) { p->v = __builtin_bit_cast(uint16_t, __bf16(v)); }
 __device__ inline void store_out(uint16_t* p, float v) { *p = __builtin_bit_cast(uint16_t, _Float16(v)); }
 
 template <typename TOut>
@@ -84,7 +86,7 @@ struct GemmArgs16 {
 
 // Copy a column-major rows x cols matrix of 16-bit elements (leading dimension ld_src, any alignment) into a
 // 16-byte aligned buffer with leading dimension ld_dst (a multiple of 8, >= rows); rows .. ld_dst - 1 are zeros.
-__global__ void __launch_bounds__(256)
+static __global__ void __launch_bounds__(256)
     copy_pad16_kernel(const uint16_t* __restrict__ src, int64_t ld_src, uint16_t* __restrict__ dst, int64_t ld_dst,
                       int64_t rows, int64_t cols) {
   typedef u16x8 u16x8_any __attribute__((aligned(2)));
@@ -507,7 +509,7 @@ __global__ void __launch_bounds__(256) gemm_block16_kernel(const GemmArgs16<TOut
 }
 
 // C = beta * C for 16-bit output (alpha == 0 path): multiply in fp32, round once.
-__global__ void __launch_bounds__(256)
+static __global__ void __launch_bounds__(256)
     scale_matrix16_kernel(uint16_t* c, int64_t rows, int64_t cols, int64_t ld, int64_t stride, int64_t batch,
                           float beta, int assign_zero) {
   const int64_t per = rows * cols;

@@ -1071,8 +1071,13 @@ __device__ inline void store_tiles(bool read_c, V beta, PtrF&& ptr, ValF&& value
     }
 }
 
+// bfloat16 in memory as an output type of its own (uint16_t outputs are halves).
+struct bf16_bits {
+  uint16_t v;
+};
+
 // The same epilogue for a wavefront tile that lies wholly inside C (elements of 2, 4 or 8 bytes in memory; 2-byte
-// elements are halves, widened to / rounded from the float the arithmetic runs in).  Addresses are a
+// elements are halves or bfloat16, widened to / rounded from the float the arithmetic runs in).  Addresses are a
 // wave-uniform buffer descriptor at the tile's origin, one 32-bit per-lane byte offset (the lane's row and its
 // share of the column index) and a scalar offset per element (the rest of the column index times ldc): no
 // 64-bit address per element, no exec-mask branch.  With C read, the loads of the next batch of 16 (8-byte
@@ -1084,7 +1089,7 @@ template <int MI, int NI, int NACC, int MT, typename V, typename TMem, typename 
 __device__ inline void store_tiles_interior(bool read_c, V beta, TMem* origin, int64_t ldc, int lane_row, int lane_col,
                                             ColF&& col_of, ValF&& value) {
   typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
-  static_assert(sizeof(TMem) == sizeof(V) || (sizeof(TMem) == 2 && sizeof(V) == 4), "same type, or halves behind floats");
+  static_assert(sizeof(TMem) == sizeof(V) || (sizeof(TMem) == 2 && sizeof(V) == 4), "same type, or 16-bit elements behind floats");
   static_assert(sizeof(V) == 4 || sizeof(V) == 8, "4- or 8-byte arithmetic");
   constexpr int E = MI * NI * NACC;
   // elements per batch: 16 four-byte or 8 eight-byte loads in flight, less where the tile does not divide that way
@@ -1104,7 +1109,8 @@ __device__ inline void store_tiles_interior(bool read_c, V beta, TMem* origin, i
   auto load = [&](int e) -> V {
     if constexpr (sizeof(TMem) == 2) {
       const unsigned short h = __builtin_amdgcn_raw_buffer_load_b16(rc, voff(e), soff(e), 0);
-      return V(__builtin_bit_cast(_Float16, h));
+      if constexpr (std::is_same<TMem, bf16_bits>::value) return V(__builtin_bit_cast(float, uint32_t(h) << 16));
+      else return V(__builtin_bit_cast(_Float16, h));
     } else if constexpr (sizeof(V) == 4) {
       return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b32(rc, voff(e), soff(e), 0));
     } else {
@@ -1112,7 +1118,9 @@ __device__ inline void store_tiles_interior(bool read_c, V beta, TMem* origin, i
     }
   };
   auto store = [&](int e, V v) {
-    if constexpr (sizeof(TMem) == 2)
+    if constexpr (std::is_same<TMem, bf16_bits>::value)
+      __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, __bf16(v)), rc, voff(e), soff(e), 0);
+    else if constexpr (sizeof(TMem) == 2)
       __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, _Float16(v)), rc, voff(e), soff(e), 0);
     else if constexpr (sizeof(V) == 4)
       __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned int, v), rc, voff(e), soff(e), 0);

@@ -1,0 +1,315 @@
+// C ABI of the feed-forward entry points (include/sbamd_ffn.h): argument rules, repacking, launches.
+#include <cctype>
+#include <string>
+
+#include "gemm_dispatch.hpp"
+#include "gemm_ffn.hpp"
+
+namespace sbamd {
+namespace {
+
+int ffn_fail(Handle* h, hipError_t e, const char* what) {
+  if (e == hipErrorNotSupported) return SBAMD_NOT_SUPPORTED;
+  h->last_error = std::string(what) + ": " + hipGetErrorString(e);
+  return e == hipErrorOutOfMemory ? SBAMD_ALLOC_FAILED : SBAMD_HIP_ERROR;
+}
+
+void forget_last(Handle* h, int64_t k) {
+  h->last_kernel = -1;
+  h->last_depth = 1;
+  h->last_k_chunk = k;
+  h->last_tile_m = h->last_tile_n = 0;
+  h->last_fused = false;
+}
+
+// 'n' -> 0, 't' / 'c' -> 1, anything else -> -1
+int trans_of(char t) {
+  const char c = char(std::tolower(static_cast<unsigned char>(t)));
+  return c == 'n' ? 0 : c == 't' || c == 'c' ? 1 : -1;
+}
+
+template <typename Tag, typename TOut, bool GATED, int NB, int DEPTH>
+hipError_t launch_narrow(FfnArgs<TOut> g, hipStream_t stream) {
+  auto kernel = ffn_narrow_kernel<Tag, TOut, GATED, NB, DEPTH>;
+  constexpr int lds = narrow_lds_bytes<NB>();
+  static_assert(lds <= 64 * 1024, "within the default limit of dynamic LDS");
+  const int64_t tm = ceil_div(g.m, GATED ? NARROW_ROWS / 2 : NARROW_ROWS), tn = ceil_div(g.n, 16 * NB);
+  if (tm > 0x7fffffffLL / tn) return hipErrorInvalidValue;
+  g.tiles_m = int32_t(tm);
+  g.tiles_n = int32_t(tn);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(NARROW_WAVES * 64), lds, stream, g);
+  return hipGetLastError();
+}
+
+// An operand as the caller has it, and what the kernels read.
+struct Rows {
+  const void* x;
+  int64_t ld;     // elements
+  int64_t rows, k;
+  bool across;    // element (row, k) at row + k * ld instead of k + row * ld
+};
+
+template <int BYTES>
+hipError_t pack(Handle* h, const Rows& o, unsigned char* dst, int64_t row_bytes) {
+  const unsigned char* src = static_cast<const unsigned char*>(o.x);
+  const int64_t grid = o.across ? ceil_div(o.rows, 64) * ceil_div(row_bytes / BYTES, 64) : ceil_div(row_bytes / 16 * o.rows, 256);
+  if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
+  if (o.across)
+    hipLaunchKernelGGL((ffn_pack_kernel<BYTES, true>), dim3((unsigned)grid), dim3(256), 0, h->stream, src, o.ld, dst, row_bytes, o.rows, o.k);
+  else
+    hipLaunchKernelGGL((ffn_pack_kernel<BYTES, false>), dim3((unsigned)grid), dim3(256), 0, h->stream, src, o.ld, dst, row_bytes, o.rows, o.k);
+  return hipGetLastError();
+}
+
+// The product behind all forward entry points.  Operands that do not lie along k are repacked into the handle's second
+// scratch area first.
+template <typename Tag, typename TOut, bool GATED>
+hipError_t run_ffn(Handle* h, const Rows& a, const Rows& b, FfnArgs<TOut> g) {
+  constexpr int BYTES = FfnMma<Tag>::BYTES;
+  const int64_t row_bytes = ceil_div(a.k * BYTES, 64) * 64;
+  const size_t bytes_a = a.across ? size_t(a.rows) * size_t(row_bytes) : 0, bytes_b = b.across ? size_t(b.rows) * size_t(row_bytes) : 0;
+  g.a = static_cast<const unsigned char*>(a.x), g.lda = a.ld * BYTES;
+  g.b = static_cast<const unsigned char*>(b.x), g.ldb = b.ld * BYTES;
+  g.kb = a.k * BYTES;
+  if (bytes_a + bytes_b > 0) {
+    hipError_t e = ensure_aux(h, bytes_a + bytes_b);  // (rows of 64 bytes: b stays aligned behind a)
+    if (e != hipSuccess) return e;
+    unsigned char* at = static_cast<unsigned char*>(h->aux);
+    if (a.across) {
+      if ((e = pack<BYTES>(h, a, at, row_bytes)) != hipSuccess) return e;
+      g.a = at, g.lda = row_bytes;
+    }
+    if (b.across) {
+      if ((e = pack<BYTES>(h, b, at + bytes_a, row_bytes)) != hipSuccess) return e;
+      g.b = at + bytes_a, g.ldb = row_bytes;
+    }
+  }
+  h->last_kernel = SBAMD_KERNEL_SMALL;
+  if (g.n <= 16) return launch_narrow<Tag, TOut, GATED, 1, 4>(g, h->stream);
+  if (g.n <= 32) return launch_narrow<Tag, TOut, GATED, 2, 4>(g, h->stream);
+  return launch_narrow<Tag, TOut, GATED, 4, 2>(g, h->stream);
+}
+
+// ------------------------------------------------------------------ front ends
+template <typename TOut>
+hipError_t scale_c(Handle* h, TOut* c, int64_t m, int64_t n, int64_t ldc, float beta);
+template <>
+hipError_t scale_c<float>(Handle* h, float* c, int64_t m, int64_t n, int64_t ldc, float beta) {
+  return run_scale_f32(h, c, m, n, ldc, 0, 1, beta, beta == 0.0f);
+}
+template <>
+hipError_t scale_c<uint16_t>(Handle* h, uint16_t* c, int64_t m, int64_t n, int64_t ldc, float beta) {
+  return run_scale_f16(h, c, m, n, ldc, 0, 1, beta, beta == 0.0f);
+}
+__global__ void __launch_bounds__(256) ffn_scale_bf16_kernel(bf16_bits* c, int64_t m, int64_t n, int64_t ldc, float beta, int beta_zero) {
+  const int64_t idx = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (idx >= m * n) return;
+  bf16_bits* p = c + idx % m + idx / m * ldc;
+  store_out(p, beta_zero ? 0.0f : beta * load_out(p));
+}
+template <>
+hipError_t scale_c<bf16_bits>(Handle* h, bf16_bits* c, int64_t m, int64_t n, int64_t ldc, float beta) {
+  const int64_t grid = ceil_div(m * n, 256);
+  if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(ffn_scale_bf16_kernel, dim3((unsigned)grid), dim3(256), 0, h->stream, c, m, n, ldc, beta, beta == 0.0f ? 1 : 0);
+  return hipGetLastError();
+}
+
+// Sizes and leading dimensions shared by the forward entry points; SBAMD_OK and `done` when there is nothing to write.
+int check_sizes(int ta, int tb, int64_t rows_a, int64_t m, int64_t n, int64_t k, int64_t lda, int64_t ldb, int64_t ldc) {
+  (void)m;
+  if (lda < (ta ? k : rows_a) || ldb < (tb ? n : k) || ldc < m) return SBAMD_INVALID_VALUE;
+  return SBAMD_OK;
+}
+
+template <typename Tag, typename TOut, bool GATED>
+int forward(sbamd_handle_t hh, int act, char transa, char transb, int64_t m, int64_t n, int64_t k, float alpha, const void* a,
+            int64_t lda, const float* scale_a, const void* b, int64_t ldb, const float* scale_b, float beta, TOut* c, int64_t ldc,
+            TOut* p, int64_t ldp) {
+  if (!hh) return SBAMD_INVALID_HANDLE;
+  Handle* h = &hh->impl;
+  // (2m and byte counts along k have to fit 63 bits)
+  constexpr int64_t LIMIT = int64_t(1) << 40;
+  if (m < 0 || n < 0 || k < 0 || m > LIMIT || n > LIMIT || k > LIMIT) return SBAMD_INVALID_VALUE;
+  if (GATED && (act < SBAMD_ACT_SILU || act > SBAMD_ACT_RELU)) return SBAMD_INVALID_VALUE;
+  DeviceGuard guard(h->device);
+  if (!guard.ok) return SBAMD_HIP_ERROR;
+  forget_last(h, k);
+  if (!GATED && alpha == 0.0f) {  // as in GEMM: before the trans flags, A and B are not read
+    if (m == 0 || n == 0) return SBAMD_OK;
+    if (!c || ldc < m) return SBAMD_INVALID_VALUE;
+    if (beta == 1.0f) return SBAMD_OK;
+    const hipError_t e = scale_c<TOut>(h, c, m, n, ldc, beta);
+    return e == hipSuccess ? SBAMD_OK : ffn_fail(h, e, "scale launch");
+  }
+  const int ta = trans_of(transa), tb = trans_of(transb);
+  if (ta < 0) return SBAMD_INVALID_TRANSA;
+  if (tb < 0) return SBAMD_INVALID_TRANSB;
+  if (std::is_same<Tag, I8Tag>::value && k > SBAMD_I8_MAX_K) return SBAMD_NOT_SUPPORTED;
+  const int64_t rows_a = GATED ? 2 * m : m;
+  if (check_sizes(ta, tb, rows_a, m, n, k, lda, ldb, ldc) != SBAMD_OK) return SBAMD_INVALID_VALUE;
+  if (GATED && p && ldp < 2 * m) return SBAMD_INVALID_VALUE;
+  if (m == 0 || n == 0) return SBAMD_OK;
+  if (!c || (k > 0 && (!a || !b))) return SBAMD_INVALID_VALUE;
+  FfnArgs<TOut> g;
+  g.m = m, g.n = n;
+  g.scale_a = scale_a, g.scale_b = scale_b;
+  g.c = c, g.ldc = ldc;
+  g.p = p, g.ldp = ldp;
+  g.alpha = alpha, g.beta = beta, g.beta_zero = beta == 0.0f ? 1 : 0;
+  g.act = act;
+  const Rows ra = {a, lda, rows_a, k, ta == 0}, rb = {b, ldb, n, k, tb != 0};
+  const hipError_t e = run_ffn<Tag, TOut, GATED>(h, ra, rb, g);
+  return e == hipSuccess ? SBAMD_OK : ffn_fail(h, e, "feed-forward launch");
+}
+
+template <typename Tag, int TPC, int HOLD>
+hipError_t launch_quantize(Handle* h, int64_t m, int64_t n, const typename QuantIn<Tag>::type* x, int64_t ldx, int8_t* q, int64_t ldq,
+                           float* scale) {
+  constexpr int COLS = TPC < 256 ? 256 / TPC : 1;
+  const int64_t grid = ceil_div(n, COLS);
+  if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((ffn_quantize_kernel<Tag, TPC, HOLD>), dim3((unsigned)grid), dim3(TPC < 256 ? 256 : TPC), 0, h->stream, m, n, x, ldx, q,
+                     ldq, scale);
+  return hipGetLastError();
+}
+
+template <typename Tag>
+int quantize(sbamd_handle_t hh, int64_t m, int64_t n, const typename QuantIn<Tag>::type* x, int64_t ldx, int8_t* q, int64_t ldq,
+             float* scale) {
+  if (!hh) return SBAMD_INVALID_HANDLE;
+  Handle* h = &hh->impl;
+  if (m < 0 || n < 0 || ldx < m || ldq < m) return SBAMD_INVALID_VALUE;
+  DeviceGuard guard(h->device);
+  if (!guard.ok) return SBAMD_HIP_ERROR;
+  forget_last(h, 0);
+  if (n == 0) return SBAMD_OK;
+  if (!scale || (m > 0 && (!x || !q))) return SBAMD_INVALID_VALUE;
+  hipError_t e;
+  if (m <= 64 * 8) e = launch_quantize<Tag, 64, 1>(h, m, n, x, ldx, q, ldq, scale);
+  else if (m <= 256 * 8 * 2) e = launch_quantize<Tag, 256, 2>(h, m, n, x, ldx, q, ldq, scale);
+  else e = launch_quantize<Tag, 1024, 2>(h, m, n, x, ldx, q, ldq, scale);
+  return e == hipSuccess ? SBAMD_OK : ffn_fail(h, e, "quantise launch");
+}
+
+// C of type TOut = alpha op(A) op(B) + beta C on the 16-bit GEMM back end, single product.
+template <typename TOut>
+Problem<uint16_t, TOut> product(bool ta, bool tb, int64_t m, int64_t n, int64_t k, const uint16_t* a, int64_t lda, const uint16_t* b,
+                                int64_t ldb, float beta, TOut* c, int64_t ldc) {
+  Problem<uint16_t, TOut> q{};
+  q.ta = ta, q.tb = tb, q.m = m, q.n = n, q.k = k;
+  q.a = a, q.lda = lda, q.b = b, q.ldb = ldb, q.c = c, q.ldc = ldc;
+  q.batch = 1;
+  q.beta_zero = beta == 0.0f;
+  return q;
+}
+hipError_t run_product(Handle* h, const Problem<uint16_t, uint16_t>& q, float beta) { return run_gemm_h(h, q, 1.0f, beta); }
+hipError_t run_product(Handle* h, const Problem<uint16_t, bf16_bits>& q, float beta) { return run_gemm_b(h, q, 1.0f, beta); }
+
+template <typename Tag, typename TOut>
+int gradient(sbamd_handle_t hh, int act, char transa, char transb, int64_t m, int64_t n, int64_t k, const uint16_t* a, int64_t lda,
+             const uint16_t* b, int64_t ldb, const uint16_t* p, int64_t ldp, const uint16_t* dc, int64_t lddc, uint16_t* dp,
+             int64_t lddp, float beta_a, uint16_t* da, int64_t ldda, float beta_b, uint16_t* db, int64_t lddb) {
+  if (!hh) return SBAMD_INVALID_HANDLE;
+  Handle* h = &hh->impl;
+  constexpr int64_t LIMIT = int64_t(1) << 40;
+  if (m < 0 || n < 0 || k < 0 || m > LIMIT || n > LIMIT || k > LIMIT) return SBAMD_INVALID_VALUE;
+  if (act < SBAMD_ACT_SILU || act > SBAMD_ACT_RELU) return SBAMD_INVALID_VALUE;
+  DeviceGuard guard(h->device);
+  if (!guard.ok) return SBAMD_HIP_ERROR;
+  forget_last(h, k);
+  const int ta = trans_of(transa), tb = trans_of(transb);
+  if (ta < 0) return SBAMD_INVALID_TRANSA;
+  if (tb < 0) return SBAMD_INVALID_TRANSB;
+  const int64_t rows_a = ta ? k : 2 * m, rows_b = tb ? n : k;
+  if (ldp < 2 * m || lddc < m || lddp < 2 * m || (da && ldda < rows_a) || (db && lddb < rows_b)) return SBAMD_INVALID_VALUE;
+  if ((da && ldb < rows_b) || (db && lda < rows_a)) return SBAMD_INVALID_VALUE;
+  const bool tokens = m > 0 && n > 0;  // is there a dP at all?
+  if (tokens && (!p || !dc || !dp)) return SBAMD_INVALID_VALUE;
+  if (dp == p && lddp != ldp) return SBAMD_INVALID_VALUE;  // in place means element for element
+  if (tokens && k > 0 && ((da && !b) || (db && !a))) return SBAMD_INVALID_VALUE;
+  if (tokens) {
+    const int64_t grid = ceil_div(ceil_div(m, 8) * n, 256);
+    if (grid > 0x7fffffffLL) return SBAMD_INVALID_VALUE;
+    hipLaunchKernelGGL((ffn_gate_grad_kernel<Tag, TOut>), dim3((unsigned)grid), dim3(256), 0, h->stream, act, m, n, p, ldp, dc, lddc, dp, lddp);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return ffn_fail(h, e, "gradient launch");
+  }
+  // The products run with n (m) == 0 too: a sum over nothing is beta times what was there.
+  if (da && m > 0 && k > 0) {
+    TOut* out = reinterpret_cast<TOut*>(da);
+    const hipError_t e = ta ? run_product(h, product<TOut>(tb, true, k, 2 * m, n, b, ldb, dp, lddp, beta_a, out, ldda), beta_a)
+                            : run_product(h, product<TOut>(false, !tb, 2 * m, k, n, dp, lddp, b, ldb, beta_a, out, ldda), beta_a);
+    if (e != hipSuccess) return ffn_fail(h, e, "gradient product");
+  }
+  if (db && n > 0 && k > 0) {
+    TOut* out = reinterpret_cast<TOut*>(db);
+    const hipError_t e = tb ? run_product(h, product<TOut>(true, ta, n, k, 2 * m, dp, lddp, a, lda, beta_b, out, lddb), beta_b)
+                            : run_product(h, product<TOut>(!ta, false, k, n, 2 * m, a, lda, dp, lddp, beta_b, out, lddb), beta_b);
+    if (e != hipSuccess) return ffn_fail(h, e, "gradient product");
+  }
+  return SBAMD_OK;
+}
+
+}  // namespace
+}  // namespace sbamd
+
+using namespace sbamd;
+
+extern "C" {
+
+int sbamd_squantize_i8(sbamd_handle_t h, int64_t m, int64_t n, const float* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale) {
+  return quantize<F32Tag>(h, m, n, x, ldx, q, ldq, scale);
+}
+int sbamd_hquantize_i8(sbamd_handle_t h, int64_t m, int64_t n, const uint16_t* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale) {
+  return quantize<HalfTag>(h, m, n, x, ldx, q, ldq, scale);
+}
+int sbamd_bquantize_i8(sbamd_handle_t h, int64_t m, int64_t n, const uint16_t* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale) {
+  return quantize<Bf16Tag>(h, m, n, x, ldx, q, ldq, scale);
+}
+
+#define SBAMD_SCALED(NAME, COUT, TOUT)                                                                                          \
+  int NAME(sbamd_handle_t h, char transa, char transb, int64_t m, int64_t n, int64_t k, float alpha, const int8_t* a,           \
+           int64_t lda, const float* scale_a, const int8_t* b, int64_t ldb, const float* scale_b, float beta, COUT* c,          \
+           int64_t ldc) {                                                                                                       \
+    return forward<I8Tag, TOUT, false>(h, SBAMD_ACT_SILU, transa, transb, m, n, k, alpha, a, lda, scale_a, b, ldb, scale_b,     \
+                                       beta, reinterpret_cast<TOUT*>(c), ldc, nullptr, 0);                                      \
+  }
+SBAMD_SCALED(sbamd_i8sgemm, float, float)
+SBAMD_SCALED(sbamd_i8hgemm, uint16_t, uint16_t)
+SBAMD_SCALED(sbamd_i8bgemm, uint16_t, bf16_bits)
+#undef SBAMD_SCALED
+
+#define SBAMD_GATED(NAME, TAG, TOUT)                                                                                            \
+  int NAME(sbamd_handle_t h, int act, char transa, char transb, int64_t m, int64_t n, int64_t k, const uint16_t* a,             \
+           int64_t lda, const uint16_t* b, int64_t ldb, uint16_t* c, int64_t ldc, uint16_t* p, int64_t ldp) {                   \
+    return forward<TAG, TOUT, true>(h, act, transa, transb, m, n, k, 1.0f, a, lda, nullptr, b, ldb, nullptr, 0.0f,              \
+                                    reinterpret_cast<TOUT*>(c), ldc, reinterpret_cast<TOUT*>(p), ldp);                          \
+  }
+SBAMD_GATED(sbamd_hgated_gemm, HalfTag, uint16_t)
+SBAMD_GATED(sbamd_bgated_gemm, Bf16Tag, bf16_bits)
+#undef SBAMD_GATED
+
+#define SBAMD_GATED_I8(NAME, COUT, TOUT)                                                                                        \
+  int NAME(sbamd_handle_t h, int act, char transa, char transb, int64_t m, int64_t n, int64_t k, const int8_t* a,               \
+           int64_t lda, const float* scale_a, const int8_t* b, int64_t ldb, const float* scale_b, COUT* c, int64_t ldc) {       \
+    return forward<I8Tag, TOUT, true>(h, act, transa, transb, m, n, k, 1.0f, a, lda, scale_a, b, ldb, scale_b, 0.0f,            \
+                                      reinterpret_cast<TOUT*>(c), ldc, nullptr, 0);                                             \
+  }
+SBAMD_GATED_I8(sbamd_i8sgated_gemm, float, float)
+SBAMD_GATED_I8(sbamd_i8hgated_gemm, uint16_t, uint16_t)
+SBAMD_GATED_I8(sbamd_i8bgated_gemm, uint16_t, bf16_bits)
+#undef SBAMD_GATED_I8
+
+#define SBAMD_GRAD(NAME, TAG, TOUT)                                                                                             \
+  int NAME(sbamd_handle_t h, int act, char transa, char transb, int64_t m, int64_t n, int64_t k, const uint16_t* a,             \
+           int64_t lda, const uint16_t* b, int64_t ldb, const uint16_t* p, int64_t ldp, const uint16_t* dc, int64_t lddc,       \
+           uint16_t* dp, int64_t lddp, float beta_a, uint16_t* da, int64_t ldda, float beta_b, uint16_t* db, int64_t lddb) {    \
+    return gradient<TAG, TOUT>(h, act, transa, transb, m, n, k, a, lda, b, ldb, p, ldp, dc, lddc, dp, lddp, beta_a, da, ldda,   \
+                               beta_b, db, lddb);                                                                               \
+  }
+SBAMD_GRAD(sbamd_hgated_gemm_grad, HalfTag, uint16_t)
+SBAMD_GRAD(sbamd_bgated_gemm_grad, Bf16Tag, bf16_bits)
+#undef SBAMD_GRAD
+
+}  // extern "C"

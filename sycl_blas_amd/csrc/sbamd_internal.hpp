@@ -135,6 +135,9 @@ hipError_t run_gemm_f64(Handle* h, const Problem<double, double>& p);
 hipError_t run_gemm_h(Handle* h, const Problem<uint16_t, uint16_t>& p, float alpha, float beta);
 hipError_t run_gemm_hs(Handle* h, const Problem<uint16_t, float>& p, float alpha, float beta);
 hipError_t run_gemm_bs(Handle* h, const Problem<uint16_t, float>& p, float alpha, float beta);
+// bfloat16 -> bfloat16 (the gated block's gradients; defined with the others)
+struct bf16_bits;
+hipError_t run_gemm_b(Handle* h, const Problem<uint16_t, bf16_bits>& p, float alpha, float beta);
 hipError_t run_scale_f16(Handle* h, uint16_t* c, int64_t rows, int64_t cols, int64_t ld, int64_t stride,
                          int64_t batch, float beta, bool assign_zero);
 

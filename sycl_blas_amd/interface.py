@@ -29,6 +29,14 @@ class gemm_batch_type_t(enum.IntEnum):
     interleaved = 1
 
 
+class activation_t(enum.IntEnum):
+    """Activation of the gated block (include/sbamd_ffn.h)."""
+    silu = _lib.ACT_SILU
+    gelu = _lib.ACT_GELU
+    gelu_tanh = _lib.ACT_GELU_TANH
+    relu = _lib.ACT_RELU
+
+
 class SbamdError(RuntimeError):
     """A HIP or allocation failure reported by the library (never an argument error)."""
 
@@ -48,8 +56,8 @@ _ARG_ERRORS = {
     _lib.INVALID_STRIDEB: "invalid _strideb",
 }
 
-# storage dtype name -> (itemsize, sbamd_fill_uniform code)
-_DTYPES = {"float32": (4, 0), "float64": (8, 1), "float16": (2, 2), "bfloat16": (2, 3)}
+# storage dtype name -> (itemsize, sbamd_fill_uniform code; None: not filled by it)
+_DTYPES = {"float32": (4, 0), "float64": (8, 1), "float16": (2, 2), "bfloat16": (2, 3), "int8": (1, None)}
 
 
 def _dtype_name(dtype):
@@ -278,6 +286,8 @@ class helper:
     @staticmethod
     def fill_uniform(sb_handle, buf, count, seed, lo=-2.0, hi=5.0):
         code = _DTYPES[buf.dtype][1]
+        if code is None:
+            raise TypeError(f"fill_uniform does not fill {buf.dtype}")
         _check(sb_handle, _lib.load().sbamd_fill_uniform(sb_handle._h, buf.ptr, int(count), code,
                                                           int(seed), float(lo), float(hi)))
         return sb_handle.record_event()
@@ -382,5 +392,100 @@ def _trsm(sb_handle, side, uplo, trans, diag, M, N, alpha, A, lda, B, ldb, _depe
     sb_handle.depends_on(_dependencies)
     st = getattr(_lib.load(), f"sbamd_{prefix}trsm")(sb_handle._h, _ch(side), _ch(uplo), _ch(trans), _ch(diag), int(M),
                                                      int(N), scalar(alpha), A.ptr, int(lda), B.ptr, int(ldb))
+    _check(sb_handle, st)
+    return [sb_handle.record_event()]
+
+
+# ------------------------------------------------- feed-forward layers (include/sbamd_ffn.h; no reference counterpart)
+_FLOATS = {"float32": "s", "float16": "h", "bfloat16": "b"}
+_HALVES = {"float16": "h", "bfloat16": "b"}
+
+
+def _ptr(buf):
+    return None if buf is None else buf.ptr
+
+
+def _want(buf, dtype, what):
+    if buf is not None and buf.dtype != dtype:
+        raise TypeError(f"{what} must be {dtype}, not {buf.dtype}")
+
+
+def _quantize(sb_handle, _M, _N, x_, _ldx, q_, _ldq, scale_, _dependencies=()):
+    """Columns of the M x N matrix x to int8 with one float scale per column (sbamd_{s,h,b}quantize_i8):
+    scale = largest magnitude / 127, q = the integer nearest to x / scale."""
+    if x_.dtype not in _FLOATS:
+        raise TypeError(f"no quantisation of {x_.dtype}")
+    _want(q_, "int8", "q")
+    _want(scale_, "float32", "scale")
+    sb_handle.depends_on(_dependencies)
+    st = getattr(_lib.load(), f"sbamd_{_FLOATS[x_.dtype]}quantize_i8")(sb_handle._h, int(_M), int(_N), x_.ptr, int(_ldx), q_.ptr,
+                                                                      int(_ldq), scale_.ptr)
+    _check(sb_handle, st)
+    return [sb_handle.record_event()]
+
+
+def _gemm_scaled(sb_handle, _TransA, _TransB, _M, _N, _K, _alpha, a_, _lda, scale_a, b_, _ldb, scale_b, _beta, _C, _ldc,
+                 _dependencies=()):
+    """C <- alpha * diag(scale_a) * op(A) * op(B) * diag(scale_b) + beta * C, A and B int8 (sbamd_i8{s,h,b}gemm).
+    A scale may be None (ones)."""
+    if _C.dtype not in _FLOATS:
+        raise TypeError(f"no 8-bit product with {_C.dtype} output")
+    _want(a_, "int8", "A")
+    _want(b_, "int8", "B")
+    _want(scale_a, "float32", "scale_a")
+    _want(scale_b, "float32", "scale_b")
+    sb_handle.depends_on(_dependencies)
+    st = getattr(_lib.load(), f"sbamd_i8{_FLOATS[_C.dtype]}gemm")(
+        sb_handle._h, _ch(_TransA), _ch(_TransB), int(_M), int(_N), int(_K), _alpha, a_.ptr, int(_lda), _ptr(scale_a), b_.ptr,
+        int(_ldb), _ptr(scale_b), _beta, _C.ptr, int(_ldc))
+    _check(sb_handle, st)
+    return [sb_handle.record_event()]
+
+
+def _gated_gemm(sb_handle, act, _TransA, _TransB, _M, _N, _K, a_, _lda, b_, _ldb, _C, _ldc, p_=None, _ldp=0, _dependencies=()):
+    """C <- act(G) * U with (G; U) = op(A) * op(B), op(A) 2M x K, in one kernel (sbamd_{h,b}gated_gemm).  p_, 2M x N,
+    receives (G; U) for `_gated_gemm_grad`."""
+    if a_.dtype not in _HALVES:
+        raise TypeError(f"no gated block on {a_.dtype}")
+    for buf, what in ((b_, "B"), (_C, "C"), (p_, "P")):
+        _want(buf, a_.dtype, what)
+    sb_handle.depends_on(_dependencies)
+    st = getattr(_lib.load(), f"sbamd_{_HALVES[a_.dtype]}gated_gemm")(
+        sb_handle._h, int(act), _ch(_TransA), _ch(_TransB), int(_M), int(_N), int(_K), a_.ptr, int(_lda), b_.ptr, int(_ldb), _C.ptr,
+        int(_ldc), _ptr(p_), int(_ldp))
+    _check(sb_handle, st)
+    return [sb_handle.record_event()]
+
+
+def _gated_gemm_scaled(sb_handle, act, _TransA, _TransB, _M, _N, _K, a_, _lda, scale_a, b_, _ldb, scale_b, _C, _ldc,
+                       _dependencies=()):
+    """The gated block on int8 operands, (G; U) = diag(scale_a) * op(A) * op(B) * diag(scale_b)
+    (sbamd_i8{s,h,b}gated_gemm).  scale_a has 2M entries."""
+    if _C.dtype not in _FLOATS:
+        raise TypeError(f"no 8-bit gated block with {_C.dtype} output")
+    _want(a_, "int8", "A")
+    _want(b_, "int8", "B")
+    _want(scale_a, "float32", "scale_a")
+    _want(scale_b, "float32", "scale_b")
+    sb_handle.depends_on(_dependencies)
+    st = getattr(_lib.load(), f"sbamd_i8{_FLOATS[_C.dtype]}gated_gemm")(
+        sb_handle._h, int(act), _ch(_TransA), _ch(_TransB), int(_M), int(_N), int(_K), a_.ptr, int(_lda), _ptr(scale_a), b_.ptr,
+        int(_ldb), _ptr(scale_b), _C.ptr, int(_ldc))
+    _check(sb_handle, st)
+    return [sb_handle.record_event()]
+
+
+def _gated_gemm_grad(sb_handle, act, _TransA, _TransB, _M, _N, _K, a_, _lda, b_, _ldb, p_, _ldp, dc_, _lddc, dp_, _lddp, _beta_a, da_,
+                     _ldda, _beta_b, db_, _lddb, _dependencies=()):
+    """Gradient of `_gated_gemm` (sbamd_{h,b}gated_gemm_grad): dP from P and dC, then
+    dA <- the gradient of A + beta_a * dA and dB likewise.  da_ or db_ may be None; dp_ may be p_."""
+    if p_.dtype not in _HALVES:
+        raise TypeError(f"no gated block on {p_.dtype}")
+    for buf, what in ((a_, "A"), (b_, "B"), (dc_, "dC"), (dp_, "dP"), (da_, "dA"), (db_, "dB")):
+        _want(buf, p_.dtype, what)
+    sb_handle.depends_on(_dependencies)
+    st = getattr(_lib.load(), f"sbamd_{_HALVES[p_.dtype]}gated_gemm_grad")(
+        sb_handle._h, int(act), _ch(_TransA), _ch(_TransB), int(_M), int(_N), int(_K), _ptr(a_), int(_lda), _ptr(b_), int(_ldb),
+        p_.ptr, int(_ldp), dc_.ptr, int(_lddc), dp_.ptr, int(_lddp), _beta_a, _ptr(da_), int(_ldda), _beta_b, _ptr(db_), int(_lddb))
     _check(sb_handle, st)
     return [sb_handle.record_event()]
