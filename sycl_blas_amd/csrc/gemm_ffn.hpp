@@ -10,7 +10,7 @@
 // as long as both operands share it.
 #pragma once
 
-#include "gemm_half.hpp"
+#include "gemm_half_dma.hpp"
 #include "../../include/sbamd_ffn.h"
 
 namespace sbamd {
@@ -18,6 +18,7 @@ namespace sbamd {
 struct I8Tag {};  // 8-bit integers, 32-bit integer sums
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 // 16 bytes at any address (global memory takes a misaligned vector; the type says so to the compiler)
 typedef u16x8 u16x8_at1 __attribute__((aligned(1)));
@@ -54,6 +55,14 @@ struct FfnMma<I8Tag> {
   }
 };
 
+// 32 x 32 instruction of the ring: 64 bytes of k per two steps, like the 16-bit ones.
+template <>
+struct Mfma16<I8Tag> {
+  __device__ static inline i32x16 mma(u16x8 op0, u16x8 op1, i32x16 c) {
+    return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, op0), __builtin_bit_cast(i32x4, op1), c, 0, 0, 0);
+  }
+};
+
 template <typename TOut>
 struct FfnArgs {
   const unsigned char* a;  // [rows][k bytes], rows = m or 2m
@@ -81,42 +90,46 @@ __device__ inline float ffn_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f
 // tanh(y) = 2 sigmoid(2y) - 1, so 0.5 g (1 + tanh(y)) = g sigmoid(2y), without the cancellation for negative g.
 __device__ inline float gelu_tanh_arg2(float g) { return 1.5957691216057308f * (g + 0.044715f * g * g * g); }
 
-__device__ inline float act_value(int act, float g) {
-  switch (act) {
-    case SBAMD_ACT_SILU: return g * ffn_sigmoid(g);
-    case SBAMD_ACT_GELU: return 0.5f * g * erfcf(-0.70710678118654752f * g);  // 2 Phi(g) = erfc(-g / sqrt(2))
-    case SBAMD_ACT_GELU_TANH: return g * ffn_sigmoid(gelu_tanh_arg2(g));
-    default: return g <= 0.0f ? 0.0f : g;  // NaN stays NaN
-  }
+template <int ACT>
+__device__ inline float act_value(float g) {
+  if constexpr (ACT == SBAMD_ACT_SILU) return g * ffn_sigmoid(g);
+  else if constexpr (ACT == SBAMD_ACT_GELU) return 0.5f * g * erfcf(-0.70710678118654752f * g);  // 2 Phi(g) = erfc(-g / sqrt(2))
+  else if constexpr (ACT == SBAMD_ACT_GELU_TANH) return g * ffn_sigmoid(gelu_tanh_arg2(g));
+  else return g <= 0.0f ? 0.0f : g;  // NaN stays NaN
 }
 
 // act(g) and act'(g)
-__device__ inline void act_value_slope(int act, float g, float& value, float& slope) {
+template <int ACT>
+__device__ inline void act_value_slope(float g, float& value, float& slope) {
+  if constexpr (ACT == SBAMD_ACT_SILU) {
+    const float s = ffn_sigmoid(g);
+    value = g * s;
+    slope = s + value * (1.0f - s);
+  } else if constexpr (ACT == SBAMD_ACT_GELU) {
+    const float phi = 0.5f * erfcf(-0.70710678118654752f * g);
+    value = g * phi;
+    slope = phi + g * 0.3989422804014327f * ffn_exp(-0.5f * g * g);
+  } else if constexpr (ACT == SBAMD_ACT_GELU_TANH) {
+    // value = g s(z), z = 2 sqrt(2/pi) (g + 0.044715 g^3); slope = s + g s (1 - s) z'.  Far out s (1 - s) is 0
+    // and z' is not: the product is taken only where s (1 - s) is not 0 (0 * inf would be NaN).
+    const float s = ffn_sigmoid(gelu_tanh_arg2(g));
+    value = g * s;
+    const float bell = s * (1.0f - s);
+    slope = bell > 0.0f ? s + g * bell * (1.5957691216057308f * (1.0f + 0.134145f * g * g)) : s;
+  } else {
+    value = g <= 0.0f ? 0.0f : g;
+    slope = g > 0.0f ? 1.0f : (g == g ? 0.0f : g);
+  }
+}
+
+// f(integral_constant<int, act>): one uniform branch for a whole epilogue instead of one per element
+template <typename F>
+__device__ inline void with_act(int act, F&& f) {
   switch (act) {
-    case SBAMD_ACT_SILU: {
-      const float s = ffn_sigmoid(g);
-      value = g * s;
-      slope = s + value * (1.0f - s);
-      break;
-    }
-    case SBAMD_ACT_GELU: {
-      const float phi = 0.5f * erfcf(-0.70710678118654752f * g);
-      value = g * phi;
-      slope = phi + g * 0.3989422804014327f * ffn_exp(-0.5f * g * g);
-      break;
-    }
-    case SBAMD_ACT_GELU_TANH: {
-      // value = g s(z), z = 2 sqrt(2/pi) (g + 0.044715 g^3); slope = s + g s (1 - s) z'.  Far out s (1 - s) is 0
-      // and z' is not: the product is taken only where s (1 - s) is not 0 (0 * inf would be NaN).
-      const float s = ffn_sigmoid(gelu_tanh_arg2(g));
-      value = g * s;
-      const float bell = s * (1.0f - s);
-      slope = bell > 0.0f ? s + g * bell * (1.5957691216057308f * (1.0f + 0.134145f * g * g)) : s;
-      break;
-    }
-    default:
-      value = g <= 0.0f ? 0.0f : g;
-      slope = g > 0.0f ? 1.0f : (g == g ? 0.0f : g);
+    case SBAMD_ACT_SILU: f(std::integral_constant<int, SBAMD_ACT_SILU>{}); break;
+    case SBAMD_ACT_GELU: f(std::integral_constant<int, SBAMD_ACT_GELU>{}); break;
+    case SBAMD_ACT_GELU_TANH: f(std::integral_constant<int, SBAMD_ACT_GELU_TANH>{}); break;
+    default: f(std::integral_constant<int, SBAMD_ACT_RELU>{});
   }
 }
 
@@ -129,9 +142,9 @@ __device__ inline float ffn_scaled(Sum s, float sa, float sb) {
 
 // ------------------------------------------------------------- narrow kernel
 // C for a block of 32 operand rows (32 channels, or 16 gates with their 16 partners) and 16 * NB tokens.  The W
-// wavefronts of the workgroup share out k in chunks of 128 bytes (chunk c goes to wavefront c % W: together they walk W
-// whole cache lines of each row at a time) and join their sums through LDS in wavefront order, so few rows still put many
-// loads in flight and no second launch and no workspace is needed.  A wavefront's chunk goes global -> registers
+// wavefronts of the workgroup share out k in chunks of 128 bytes (a cache line of each row) and join their sums through
+// LDS in wavefront order, so few rows still put many loads in flight and neither a second launch nor a workspace is
+// needed.  A wavefront's chunk goes global -> registers
 // (lane = one 16-byte piece, 8 lanes = one row's cache line; DEPTH chunks ahead) -> its own corner of LDS -> fragments:
 // the detour through LDS turns the coalesced pieces into the matrix instruction's layout.  No barrier inside the loop:
 // LDS operations of one wavefront execute in order.  Bound by the weights' way out of memory for few tokens.
@@ -148,8 +161,34 @@ constexpr int narrow_lds_bytes() {
   return stage > join ? stage : join;
 }
 
-template <typename Tag, typename TOut, bool GATED, int NB, int DEPTH>
-__global__ void __launch_bounds__(NARROW_WAVES * 64) ffn_narrow_kernel(const FfnArgs<TOut> g) {
+// The first `have` of 16 bytes at p, zeros behind them, without reading past them: the 16 bytes that END there, shifted down
+// (all of them lie inside the row when the row has 16 bytes at all), byte by byte in a shorter row.  One load and a
+// shift for each piece instead of up to 16 dependent loads.
+__device__ inline u16x8 partial_piece(const unsigned char* p, int have, bool long_row) {
+  typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+  typedef u64x2 u64x2_at1 __attribute__((aligned(1)));
+  u64x2 v = {0, 0};
+  if (have > 0) {
+    const int drop = have < 16 ? 16 - have : 0;  // bytes of the load in front of p
+    if (long_row) {
+      v = *reinterpret_cast<const u64x2_at1*>(p - drop);
+      const int bits = drop * 8;
+      if (bits >= 64) {
+        v[0] = v[1] >> (bits - 64);
+        v[1] = 0;
+      } else if (bits > 0) {
+        v[0] = (v[0] >> bits) | (v[1] << (64 - bits));
+        v[1] = v[1] >> bits;
+      }
+    } else {
+      for (int e = 0; e < have; ++e) v[e >> 3] |= uint64_t(p[e]) << (8 * (e & 7));
+    }
+  }
+  return __builtin_bit_cast(u16x8, v);
+}
+
+template <typename Tag, typename TOut, bool GATED, int NB, int DEPTH, int OCC>
+__global__ void __launch_bounds__(NARROW_WAVES * 64, OCC) ffn_narrow_kernel(const FfnArgs<TOut> g) {
   using M = FfnMma<Tag>;
   using Sum = typename M::sum_t;
   constexpr int W = NARROW_WAVES, ROWS = NARROW_ROWS, TOK = 16 * NB;
@@ -225,18 +264,27 @@ __global__ void __launch_bounds__(NARROW_WAVES * 64) ffn_narrow_kernel(const Ffn
     __builtin_amdgcn_wave_barrier();
   };
 
-  const int64_t whole = g.kb / NARROW_CHUNK;  // whole chunks; chunk wave + W * i is this wavefront's i-th
-  const int64_t count = whole > wave ? (whole - wave + W - 1) / W : 0;
+  // Each wavefront takes a run of its own of the whole chunks and starts inside it at a place that goes by wavefront and
+  // row block: rows are often a power of two apart, and without this the rows of all workgroups walk the same few memory
+  // channels together (reading 268 MB as rows of 8192 bytes: chunks dealt out in turn 4.5 TB/s, runs 6.1, runs with turned
+  // starts 6.1; rows of 16384: 5.7 / 4.9 / 6.1; 32768: 5.4 / 5.0 / 6.0).  The order of a row's sum is fixed by its place.
+  const int64_t whole = g.kb / NARROW_CHUNK;
+  const int64_t first = whole * wave / W, count = whole * (wave + 1) / W - first;
+  const int64_t turn = count > 0 ? (int64_t(tm) * 8 + wave * 2) % count : 0;
+  auto chunk = [&](int64_t i) {
+    i += turn;
+    return first + (i < count ? i : i - count);
+  };
   const int64_t piped = count / DEPTH * DEPTH;
   // the pipelined part: no branch between a load and its use, so the compiler's waits stay counted
   if (piped > 0) {
 #pragma unroll
-    for (int d = 0; d < DEPTH; ++d) issue(reg[d], wave + int64_t(W) * d);
+    for (int d = 0; d < DEPTH; ++d) issue(reg[d], chunk(d));
     for (int64_t it = DEPTH; it < piped; it += DEPTH) {
 #pragma unroll
       for (int d = 0; d < DEPTH; ++d) {
         consume(reg[d]);
-        issue(reg[d], wave + W * (it + d));
+        issue(reg[d], chunk(it + d));
       }
     }
 #pragma unroll
@@ -245,32 +293,18 @@ __global__ void __launch_bounds__(NARROW_WAVES * 64) ffn_narrow_kernel(const Ffn
   if (piped < count) {
 #pragma unroll
     for (int d = 0; d < DEPTH - 1; ++d)
-      if (piped + d < count) issue(reg[d], wave + W * (piped + d));
+      if (piped + d < count) issue(reg[d], chunk(piped + d));
 #pragma unroll
     for (int d = 0; d < DEPTH - 1; ++d)
       if (piped + d < count) consume(reg[d]);
   }
   // the last, partial chunk: zeros behind the end of k (the rows' ends are not read past)
   const int rest = int(g.kb - whole * NARROW_CHUNK);
-  if (rest > 0 && wave == int(whole % W)) {
+  if (rest > 0 && wave == W - 1) {
     const int have = rest - piece * 16;  // bytes of this lane's piece that exist
+    const bool long_row = g.kb >= 16;
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const unsigned char* s = src[i] + whole * NARROW_CHUNK;
-      u16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
-      if (have >= 16) {
-        v = *reinterpret_cast<const u16x8_at1*>(s);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          uint16_t x = 0;
-          if (2 * e < have) x = s[2 * e];
-          if (2 * e + 1 < have) x |= uint16_t(uint16_t(s[2 * e + 1]) << 8);
-          v[e] = x;
-        }
-      }
-      reg[0][i] = v;
-    }
+    for (int i = 0; i < NL; ++i) reg[0][i] = partial_piece(src[i] + whole * NARROW_CHUNK, have, long_row);
     consume(reg[0]);
   }
 
@@ -292,25 +326,265 @@ __global__ void __launch_bounds__(NARROW_WAVES * 64) ffn_narrow_kernel(const Ffn
     for (int w = 1; w < W; ++w) s = s + part[(w * TOK + tok) * LDJ + row];
     return s;
   };
-  for (int e = tid; e < CH * TOK; e += W * 64) {
-    const int ch = e % CH, tok = e / CH;
-    const int64_t mm = m0 + ch, nn = n0 + tok;
-    if (mm >= g.m || nn >= g.n) continue;
-    const float sb = g.scale_b ? g.scale_b[nn] : 1.0f;
-    if constexpr (GATED) {
-      const float gate = ffn_scaled(joined(tok, ch), g.scale_a ? g.scale_a[mm] : 1.0f, sb);
-      const float up = ffn_scaled(joined(tok, 16 + ch), g.scale_a ? g.scale_a[g.m + mm] : 1.0f, sb);
-      if (g.p) {
-        store_out(g.p + mm + nn * g.ldp, gate);
-        store_out(g.p + g.m + mm + nn * g.ldp, up);
-      }
-      store_out(g.c + mm + nn * g.ldc, act_value(g.act, gate) * up);
-    } else {
+  auto each = [&](auto&& store) {
+    for (int e = tid; e < CH * TOK; e += W * 64) {
+      const int ch = e % CH, tok = e / CH;
+      const int64_t mm = m0 + ch, nn = n0 + tok;
+      if (mm < g.m && nn < g.n) store(ch, tok, mm, nn, g.scale_b ? g.scale_b[nn] : 1.0f);
+    }
+  };
+  if constexpr (GATED) {
+    with_act(g.act, [&](auto act) {
+      each([&](int ch, int tok, int64_t mm, int64_t nn, float sb) {
+        const float gate = ffn_scaled(joined(tok, ch), g.scale_a ? g.scale_a[mm] : 1.0f, sb);
+        const float up = ffn_scaled(joined(tok, 16 + ch), g.scale_a ? g.scale_a[g.m + mm] : 1.0f, sb);
+        if (g.p) {
+          store_out(g.p + mm + nn * g.ldp, gate);
+          store_out(g.p + g.m + mm + nn * g.ldp, up);
+        }
+        store_out(g.c + mm + nn * g.ldc, act_value<decltype(act)::value>(gate) * up);
+      });
+    });
+  } else {
+    each([&](int ch, int tok, int64_t mm, int64_t nn, float sb) {
       TOut* at = g.c + mm + nn * g.ldc;
       float out = g.alpha * ffn_scaled(joined(tok, ch), g.scale_a ? g.scale_a[mm] : 1.0f, sb);
       if (!g.beta_zero) out = out + g.beta * load_out(at);
       store_out(at, out);
+    });
+  }
+}
+
+// --------------------------------------------------------------- ring kernel
+// The 16-bit GEMM's ring (gemm_half_dma.hpp: operand tiles straight into LDS through five stages, 256 x 256 tiles on eight
+// wavefronts or 128 x 128 on four) with the feed-forward epilogue.  8-bit operands run through it as pairs: 64 bytes of
+// k per stage and row, the same pieces and fragments, half the steps for the same k.  GATED: the rows of A alternate 32 gates
+// and their 32 partners, so both halves of a channel meet in one lane and P never leaves the kernel unless asked for.
+//
+// The grid is as many workgroups as the chip holds and each walks its tiles.  The first loads of the next tile (stages
+// 0 .. 3) are issued before the epilogue of the current one, which works in the last stage alone: with a tile per workgroup
+// the unit stood still for about 10 us per 256 x 256 tile (launch, first loads, epilogue), of 35 for k = 1024.
+//
+// Epilogue: a lane holds one token and runs of four channels; they go through the wavefront's corner of LDS ([32 tokens][128
+// bytes], 16-byte piece c of row r at c ^ ((r >> 1) & 7)) and leave as whole rows of up to 128 bytes (element by element where
+// C's rows are not 16-byte aligned or the tile hangs over the edge).  16-bit results are rounded on the way into the
+// corner; with beta * C to add they stay float there and are rounded once behind the addition.
+constexpr int CORNER_ROW = 128, CORNER_BYTES = 32 * CORNER_ROW;
+__device__ inline int corner_at(int row, int byte) { return row * CORNER_ROW + (((byte >> 4) ^ ((row >> 1) & 7)) << 4) + (byte & 15); }
+
+// 32 tokens x SLAB channels of SB-byte elements (2: already of type TOut; 4: floats) from the corner to rows of `out`.
+template <int SB, int SLAB, typename TOut>
+__device__ inline void corner_to_rows(const SBAMD_LDS unsigned char* corner, TOut* out, int64_t ld, int64_t ch0, int64_t ch_lim, int64_t t0,
+                                      int64_t t_lim, bool vec, int lane, bool read_c, float beta) {
+  constexpr int V = 16 / SB, PER = SLAB / V, ROWS = 64 / PER;  // channels per piece, pieces per row, rows per instruction
+  typedef unsigned int piece_t __attribute__((ext_vector_type(V * sizeof(TOut) / 4)));
+  if (vec && ch0 + SLAB <= ch_lim) {
+    const int piece = lane % PER;
+#pragma unroll
+    for (int r = 0; r < 32; r += ROWS) {
+      const int row = r + lane / PER;
+      if (t0 + row >= t_lim) continue;
+      TOut* at = out + ch0 + piece * V + (t0 + row) * ld;
+      const i32x4 raw = *reinterpret_cast<const SBAMD_LDS i32x4*>(corner + corner_at(row, piece * 16));
+      if constexpr (SB == 2) {
+        *reinterpret_cast<i32x4*>(at) = raw;
+      } else {
+        union {
+          TOut e[V];
+          piece_t q;
+        } x;
+        f32x4_t v = __builtin_bit_cast(f32x4_t, raw);
+        if (read_c) {
+          x.q = *reinterpret_cast<const piece_t*>(at);
+#pragma unroll
+          for (int e = 0; e < V; ++e) v[e] = v[e] + beta * load_out(&x.e[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) store_out(&x.e[e], v[e]);
+        *reinterpret_cast<piece_t*>(at) = x.q;
+      }
     }
+  } else {
+    const int ch = lane % SLAB;
+    if (ch0 + ch >= ch_lim) return;
+    for (int row = lane / SLAB; row < 32 && t0 + row < t_lim; row += 64 / SLAB) {
+      TOut* at = out + ch0 + ch + (t0 + row) * ld;
+      if constexpr (SB == 2) {
+        *reinterpret_cast<uint16_t*>(at) = *reinterpret_cast<const SBAMD_LDS uint16_t*>(corner + corner_at(row, ch * 2));
+      } else {
+        float v = *reinterpret_cast<const SBAMD_LDS float*>(corner + corner_at(row, ch * 4));
+        if (read_c) v = v + beta * load_out(at);
+        store_out(at, v);
+      }
+    }
+  }
+}
+
+template <typename Tag, typename TOut, bool GATED, bool TA, bool TB, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(WM* WN * 64, 2) ffn_ring_kernel(const FfnArgs<TOut> g) {
+  constexpr int NT = WM * WN * 64;
+  constexpr int WTM = BM / WM, WTN = BN / WN;
+  constexpr int MI = WTM / 32, NI = WTN / 32;
+  constexpr int CHW = GATED ? WTM / 2 : WTM;  // channels of C per wavefront tile
+  constexpr int CHB = GATED ? BM / 2 : BM;    // and per workgroup
+  constexpr bool SCALED = std::is_same<Tag, I8Tag>::value;
+  using OpA = RingOperand<TA, BM, NT>;
+  using OpB = RingOperand<!TB, BN, NT>;
+  using Acc = typename std::conditional<SCALED, i32x16, f32x16>::type;
+  constexpr int STAGE_BYTES = OpA::BYTES + OpB::BYTES;
+  static_assert(!GATED || MI % 2 == 0, "gates and partners in pairs");
+  static_assert(WM * WN * CORNER_BYTES <= STAGE_BYTES, "the corners fit one stage");
+  static_assert(WTM % 64 == 0, "a wavefront tile's row scales lie in whole registers");
+
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem_raw[];
+  SBAMD_LDS unsigned char* smem = (SBAMD_LDS unsigned char*)smem_raw;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave % WM, wn = wave / WM;
+
+  const int64_t lda = g.lda / 2, ldb = g.ldb / 2, k_len = g.kb / 2;  // in 16-bit units
+  const int tiles = g.tiles_m * g.tiles_n;
+  OpA oa;
+  OpB ob;
+  int64_t m0, n0;
+  float sa[WTM / 64], sb[NI];  // scales: lane's rows lane, lane + 64 of the wavefront tile; lane's token of each 32-token block
+  auto begin = [&](int tile) {
+    int tm, tn;
+    tile_coords(xcd_remap(tile, tiles), g.tiles_m, g.tiles_n, tm, tn);
+    m0 = int64_t(tm) * CHB, n0 = int64_t(tn) * BN;
+    if constexpr (GATED) oa.init_gated(reinterpret_cast<const uint16_t*>(g.a), lda, m0, g.m, tid);
+    else oa.init(reinterpret_cast<const uint16_t*>(g.a), lda, m0, g.m, tid);
+    ob.init(reinterpret_cast<const uint16_t*>(g.b), ldb, n0, g.n, tid);
+    if constexpr (SCALED) {  // (rows and tokens past the edge read the last one: they only feed what is not stored)
+#pragma unroll
+      for (int i = 0; i < WTM / 64; ++i) {
+        const int row = wm * WTM + i * 64 + lane;
+        int64_t ch = m0 + (GATED ? (row >> 6) * 32 + (row & 31) : row);
+        ch = ch < g.m ? ch : g.m - 1;
+        if (GATED && (row & 32)) ch += g.m;
+        sa[i] = g.scale_a ? g.scale_a[ch] : 1.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        const int64_t t = n0 + wn * WTN + j * 32 + (lane & 31);
+        sb[j] = g.scale_b ? g.scale_b[t < g.n ? t : g.n - 1] : 1.0f;
+      }
+    }
+    ring_start<OpA, OpB, RING_STAGES>(oa, ob, lda, ldb, int(k_len / RING_BK), smem, wave);
+  };
+
+  begin(blockIdx.x);
+  for (int tile = blockIdx.x;;) {
+    Acc acc[MI][NI];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
+    // (its first barrier lies behind every wavefront's epilogue of the tile before, so the last stage may be refilled)
+    ring_multiply<Tag, OpA, OpB, MI, NI, WTM, WTN, 0, false, RING_STAGES, true>(acc, oa, ob, lda, ldb, k_len, smem, tid, lane, wave, wm, wn);
+
+    __syncthreads();  // every wavefront is through with the ring's stages
+    const int64_t ch0 = m0 + wm * CHW, tok0 = n0 + wn * WTN;
+    float sa_now[WTM / 64], sb_now[NI];
+    if constexpr (SCALED) {
+#pragma unroll
+      for (int i = 0; i < WTM / 64; ++i) sa_now[i] = sa[i];
+#pragma unroll
+      for (int j = 0; j < NI; ++j) sb_now[j] = sb[j];
+    }
+    const int next = tile + int(gridDim.x);
+    if (next < tiles) begin(next);
+
+    // The epilogue's addresses are made from a lane index the compiler cannot see through: it would otherwise compute them
+    // all in front of the tile loop and spill them.
+    int lane_e = lane;
+    asm volatile("" : "+v"(lane_e));
+    SBAMD_LDS unsigned char* corner = smem + (RING_STAGES - 1) * STAGE_BYTES + wave * CORNER_BYTES;
+    const int tok = lane_e & 31, half = lane_e >> 5;
+    auto settle = [] {  // between the lanes' writes and other lanes' reads (one wavefront: LDS keeps its order)
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    };
+    // the four floats of rows 8 Q + 4 half .. + 3 of the wavefront tile's 32-row block I, tokens of block J
+    auto four = [&](auto i_tag, auto j_tag, auto q_tag) {
+      constexpr int I = decltype(i_tag)::value, J = decltype(j_tag)::value, Q = decltype(q_tag)::value;
+      f32x4_t v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (SCALED) v[e] = ffn_scaled(acc[I][J][Q * 4 + e], __shfl(sa_now[I / 2], (I % 2) * 32 + Q * 8 + half * 4 + e, 64), sb_now[J]);
+        else v[e] = acc[I][J][Q * 4 + e];
+      }
+      return v;
+    };
+    // value(i, q) of 32-channel blocks i = B0 .. B0 + BLOCKS - 1 of the wavefront's channels, through the corner to `out`
+    auto emit = [&](auto sb_tag, auto j_tag, auto&& value, TOut* out, int64_t ld, int64_t lim, bool vec, bool read_c) {
+      constexpr int SB = decltype(sb_tag)::value, J = decltype(j_tag)::value;
+      constexpr int SLAB = CHW * SB < CORNER_ROW ? CHW : CORNER_ROW / SB, BLOCKS = SLAB / 32;
+      static_for<CHW / SLAB>([&](auto slab) {
+        constexpr int B0 = decltype(slab)::value * BLOCKS;
+        static_for<BLOCKS>([&](auto block) {
+          static_for<4>([&](auto q) {
+            const f32x4_t v = value(std::integral_constant<int, B0 + decltype(block)::value>{}, j_tag, q);
+            const int at = corner_at(tok, (decltype(block)::value * 32 + decltype(q)::value * 8 + half * 4) * SB);
+            if constexpr (SB == 4) {
+              *reinterpret_cast<SBAMD_LDS f32x4_t*>(corner + at) = v;
+            } else {
+              union {
+                TOut e[4];
+                uint64_t w;
+              } x;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) store_out(&x.e[e], v[e]);
+              *reinterpret_cast<SBAMD_LDS uint64_t*>(corner + at) = x.w;
+            }
+          });
+        });
+        settle();
+        corner_to_rows<SB, SLAB, TOut>(corner, out, ld, ch0 + decltype(slab)::value * SLAB, lim, tok0 + J * 32, g.n, vec, lane_e, read_c, g.beta);
+        settle();
+      });
+    };
+    auto rows_aligned = [](const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (ld * int64_t(sizeof(TOut))) % 16 == 0; };
+    using own_size = std::integral_constant<int, int(sizeof(TOut))>;
+    using as_float = std::integral_constant<int, 4>;
+    const bool vec_c = rows_aligned(g.c, g.ldc);
+    if constexpr (GATED) {
+      auto gate = [&](auto i, auto j, auto q) { return four(std::integral_constant<int, 2 * decltype(i)::value>{}, j, q); };
+      auto up = [&](auto i, auto j, auto q) { return four(std::integral_constant<int, 2 * decltype(i)::value + 1>{}, j, q); };
+      if (g.p) {
+        const bool vec_p = rows_aligned(g.p, g.ldp);
+        static_for<NI>([&](auto j) {
+          emit(own_size{}, j, gate, g.p, g.ldp, g.m, vec_p, false);
+          emit(own_size{}, j, up, g.p + g.m, g.ldp, g.m, vec_p && rows_aligned(g.p + g.m, g.ldp), false);
+        });
+      }
+      with_act(g.act, [&](auto act) {
+        static_for<NI>([&](auto j_tag) {
+          emit(own_size{}, j_tag, [&](auto i, auto j, auto q) {
+            const f32x4_t x = gate(i, j, q), y = up(i, j, q);
+            f32x4_t v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = act_value<decltype(act)::value>(x[e]) * y[e];
+            return v;
+          }, g.c, g.ldc, g.m, vec_c, false);
+        });
+      });
+    } else {
+      auto scaled = [&](auto i, auto j, auto q) {
+        f32x4_t v = four(i, j, q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = g.alpha * v[e];
+        return v;
+      };
+      static_for<NI>([&](auto j) {
+        if (g.beta_zero) emit(own_size{}, j, scaled, g.c, g.ldc, g.m, vec_c, false);
+        else emit(as_float{}, j, scaled, g.c, g.ldc, g.m, vec_c, true);
+      });
+    }
+    if (next >= tiles) return;
+    tile = next;
   }
 }
 
@@ -328,18 +602,8 @@ __global__ void __launch_bounds__(256)
     if (v >= per * rows) return;
     const int64_t r = v / per, at = (v - r * per) * 16, kb = k * BYTES;
     const unsigned char* s = src + r * ld * BYTES + at;
-    u16x8 out = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (at + 16 <= kb) {
-      out = *reinterpret_cast<const u16x8_at1*>(s);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        uint16_t x = 0;
-        if (at + 2 * e < kb) x = s[2 * e];
-        if (at + 2 * e + 1 < kb) x |= uint16_t(uint16_t(s[2 * e + 1]) << 8);
-        out[e] = x;
-      }
-    }
+    const int64_t left = kb - at;
+    const u16x8 out = partial_piece(s, int(left < 16 ? (left < 0 ? 0 : left) : 16), kb >= 16);
     *reinterpret_cast<u16x8*>(dst + r * row_bytes + at) = out;
   } else {
     __shared__ E tile[64][64 + 4 / BYTES];
@@ -499,9 +763,10 @@ __global__ void __launch_bounds__(256)
   const uint16_t* pg = p + col * ldp + i;
   const uint16_t* pd = dc + col * lddc + i;
   uint16_t* out = dp + col * lddp + i;
+  with_act(act, [&](auto act_tag) {
   auto one = [&](uint16_t gb, uint16_t ub, uint16_t db, uint16_t& dg, uint16_t& du) {
     float value, slope;
-    act_value_slope(act, widen(Tag{}, gb), value, slope);
+    act_value_slope<decltype(act_tag)::value>(widen(Tag{}, gb), value, slope);
     const float d = widen(Tag{}, db);
     TOut og, ou;
     store_out(&og, d * widen(Tag{}, ub) * slope);
@@ -530,6 +795,7 @@ __global__ void __launch_bounds__(256)
       out[m + e] = y;
     }
   }
+  });
 }
 
 }  // namespace sbamd

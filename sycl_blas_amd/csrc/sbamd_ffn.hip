@@ -1,5 +1,7 @@
 // C ABI of the feed-forward entry points (include/sbamd_ffn.h): argument rules, repacking, launches.
+#include <algorithm>
 #include <cctype>
+#include <cmath>
 #include <string>
 
 #include "gemm_dispatch.hpp"
@@ -28,9 +30,9 @@ int trans_of(char t) {
   return c == 'n' ? 0 : c == 't' || c == 'c' ? 1 : -1;
 }
 
-template <typename Tag, typename TOut, bool GATED, int NB, int DEPTH>
+template <typename Tag, typename TOut, bool GATED, int NB, int DEPTH, int OCC>
 hipError_t launch_narrow(FfnArgs<TOut> g, hipStream_t stream) {
-  auto kernel = ffn_narrow_kernel<Tag, TOut, GATED, NB, DEPTH>;
+  auto kernel = ffn_narrow_kernel<Tag, TOut, GATED, NB, DEPTH, OCC>;
   constexpr int lds = narrow_lds_bytes<NB>();
   static_assert(lds <= 64 * 1024, "within the default limit of dynamic LDS");
   const int64_t tm = ceil_div(g.m, GATED ? NARROW_ROWS / 2 : NARROW_ROWS), tn = ceil_div(g.n, 16 * NB);
@@ -61,33 +63,113 @@ hipError_t pack(Handle* h, const Rows& o, unsigned char* dst, int64_t row_bytes)
   return hipGetLastError();
 }
 
-// The product behind all forward entry points.  Operands that do not lie along k are repacked into the handle's second
-// scratch area first.
+template <typename Tag, typename TOut, bool GATED, bool TA, bool TB, int BM, int BN, int WM, int WN>
+hipError_t launch_ring(FfnArgs<TOut> g, int cus, hipStream_t stream) {
+  auto kernel = ffn_ring_kernel<Tag, TOut, GATED, TA, TB, BM, BN, WM, WN>;
+  constexpr int lds = ring_lds_bytes(BM, BN);
+  static PerDeviceOnce lds_limit;
+  const hipError_t e = lds_limit.run([&] {
+    return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  });
+  if (e != hipSuccess) return e;
+  const int64_t tm = ceil_div(g.m, GATED ? BM / 2 : BM), tn = ceil_div(g.n, BN);
+  // (the kernel's tile counter runs past the last tile by up to a grid)
+  if (tm > 0x7fff0000LL / tn) return hipErrorInvalidValue;
+  g.tiles_m = int32_t(tm);
+  g.tiles_n = int32_t(tn);
+  const int64_t resident = int64_t(cus) * (160 * 1024 / lds);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(tm * tn, resident)), dim3(WM * WN * 64), lds, stream, g);
+  return hipGetLastError();
+}
+
+template <typename Tag, typename TOut, bool GATED, int BM, int BN, int WM, int WN>
+hipError_t launch_ring_trans(const FfnArgs<TOut>& g, bool ta, bool tb, int cus, hipStream_t stream) {
+  // 8-bit operands always lie along k here: the transposing LDS reads the other layouts need move 16-bit elements
+  if constexpr (std::is_same<Tag, I8Tag>::value) {
+    return launch_ring<Tag, TOut, GATED, true, false, BM, BN, WM, WN>(g, cus, stream);
+  } else {
+    if (ta) return tb ? launch_ring<Tag, TOut, GATED, true, true, BM, BN, WM, WN>(g, cus, stream) : launch_ring<Tag, TOut, GATED, true, false, BM, BN, WM, WN>(g, cus, stream);
+    return tb ? launch_ring<Tag, TOut, GATED, false, true, BM, BN, WM, WN>(g, cus, stream) : launch_ring<Tag, TOut, GATED, false, false, BM, BN, WM, WN>(g, cus, stream);
+  }
+}
+
+inline bool aligned16(const void* p, int64_t ld_bytes) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld_bytes % 16 == 0; }
+
+// Which kernel: SBAMD_KERNEL_SMALL (narrow), _LARGE (128 x 128 ring) or _HUGE (256 x 256 ring), from estimated microseconds.
+// Lengths along k in bytes make one model of 8-bit and 16-bit operands: a fragment, a stage and a cache line hold the
+// same bytes, and a matrix instruction takes the same time for either.  Measured on MI355X over n = 16 ... 21504,
+// (k, m) = (1024, 4096), (4096, 1024), (4096, 4096), (4096, 16384), (16384, 4096), plain and gated:
+//   narrow: operands at 6.2 TB/s; what the workgroups (32 rows x up to 64 tokens) read again through L2 at 28 TB/s, 12
+//     where the tokens outgrow an XCD's 4 MB of it; 1.2e-3 per byte of k for a workgroup alone (rows 32768, 8192 bytes:
+//     n = 16 45 us, 48 58, 128 102; rows 8192: n = 224 43, 512 91);
+//   128 x 128: 3.3e-3 per byte of k with few tiles, 5.9e-3 with one per unit (8192 bytes: 33 / 51; 2048: 10 / 13.6), 5.5e-3
+//     per tile and unit beyond; operands at 4.4 TB/s;
+//   256 x 256: 6 us and 13e-3 per byte and round of one tile per unit (2048 bytes, 10.5 rounds: 354; 8192: 1196), 8.2e-3
+//     with few units busy.
+inline int pick_ffn(int64_t rows, int64_t n, int64_t kb, int cus, double t_ring_extra) {
+  const double len = double(kb), bytes = double(rows + n) * len;
+  const int64_t tok = n <= 16 ? 16 : n <= 32 ? 32 : n <= 48 ? 48 : 64;
+  const double blocks = double(ceil_div(n, tok));
+  const double again = (double(ceil_div(rows, NARROW_ROWS)) * blocks * double(tok) + (blocks - 1.0) * double(rows)) * len;
+  const double t_narrow = 4.0 + std::max(len * 1.2e-3, bytes / 6.2e6 + again / (double(n) * len <= 4.5e6 ? 28e6 : 12e6));
+  const double q128 = double(ceil_div(rows, 128)) * double(ceil_div(n, 128)) / cus;
+  const double t_128 = t_ring_extra + 3.0 + std::max(q128 <= 1.0 ? len * (3.3e-3 + 2.6e-3 * q128) : std::ceil(q128) * (len * 5.5e-3 + 0.7), bytes / 4.4e6);
+  const double q256 = double(ceil_div(rows, 256)) * double(ceil_div(n, 256)) / cus, whole = std::floor(q256), part = q256 - whole;
+  const double t_256 = t_ring_extra + 3.0 + whole * (6.0 + len * 13e-3) + (part > 0.0 ? 6.0 + len * (8.2e-3 + 4.5e-3 * part) : 0.0);
+  if (t_narrow <= t_128 && t_narrow <= t_256) return SBAMD_KERNEL_SMALL;
+  return t_128 <= t_256 ? SBAMD_KERNEL_LARGE : SBAMD_KERNEL_HUGE;
+}
+
+// The product behind all forward entry points.
 template <typename Tag, typename TOut, bool GATED>
 hipError_t run_ffn(Handle* h, const Rows& a, const Rows& b, FfnArgs<TOut> g) {
   constexpr int BYTES = FfnMma<Tag>::BYTES;
-  const int64_t row_bytes = ceil_div(a.k * BYTES, 64) * 64;
-  const size_t bytes_a = a.across ? size_t(a.rows) * size_t(row_bytes) : 0, bytes_b = b.across ? size_t(b.rows) * size_t(row_bytes) : 0;
-  g.a = static_cast<const unsigned char*>(a.x), g.lda = a.ld * BYTES;
-  g.b = static_cast<const unsigned char*>(b.x), g.ldb = b.ld * BYTES;
-  g.kb = a.k * BYTES;
-  if (bytes_a + bytes_b > 0) {
-    hipError_t e = ensure_aux(h, bytes_a + bytes_b);  // (rows of 64 bytes: b stays aligned behind a)
+  constexpr int STEP = RING_BK * 2;  // bytes of k per step of the ring
+  const int64_t kb = a.k * BYTES, row_bytes = ceil_div(kb, STEP) * STEP;
+  const int cus = h->compute_units > 0 ? h->compute_units : 256;
+  // What the kernel can read in place.  The narrow kernel: rows along k at any alignment.  The ring: 16-byte aligned rows
+  // of at least one step along k (8-bit: an even number), or 16-bit operands across k whose rows come in whole
+  // 16-byte pieces.  Everything else is repacked along k, zero-padded to whole steps, in the handle's second scratch area.
+  auto ring_reads = [&](const Rows& o, int64_t whole_rows) {
+    return aligned16(o.x, o.ld * BYTES) && (!o.across || (BYTES == 2 && whole_rows % 8 == 0)) && kb >= STEP && kb % 2 == 0;
+  };
+  // (the gated block's two halves of op(A) are clamped apart: m itself has to be whole pieces.  One length along k serves
+  // both operands, so a short or odd one is padded on both sides: the conditions on kb are the same for both.)
+  const bool ring_pack_a = !ring_reads(a, GATED ? a.rows / 2 : a.rows), ring_pack_b = !ring_reads(b, b.rows);
+  auto pack_time = [&](bool packed, const Rows& o) { return packed ? 3.0 + 2.0 * double(o.rows) * double(row_bytes) / 3.0e6 : 0.0; };
+  int family = h->kernel_override;
+  if (family != SBAMD_KERNEL_SMALL && family != SBAMD_KERNEL_LARGE && family != SBAMD_KERNEL_HUGE) {
+    const double extra = pack_time(ring_pack_a, a) + pack_time(ring_pack_b, b) - pack_time(a.across, a) - pack_time(b.across, b);
+    family = pick_ffn(a.rows, b.rows, kb, cus, extra);
+  }
+  if (kb == 0) family = SBAMD_KERNEL_SMALL;  // nothing to pipeline: the narrow kernel writes the sums over nothing
+  const bool ring = family != SBAMD_KERNEL_SMALL;
+  const bool pack_a = ring ? ring_pack_a : a.across, pack_b = ring ? ring_pack_b : b.across;
+  if (pack_a || pack_b) {
+    const size_t bytes_a = pack_a ? size_t(a.rows) * size_t(row_bytes) : 0, bytes_b = pack_b ? size_t(b.rows) * size_t(row_bytes) : 0;
+    const hipError_t e = ensure_aux(h, bytes_a + bytes_b);  // (rows of whole steps: b stays aligned behind a)
     if (e != hipSuccess) return e;
     unsigned char* at = static_cast<unsigned char*>(h->aux);
-    if (a.across) {
-      if ((e = pack<BYTES>(h, a, at, row_bytes)) != hipSuccess) return e;
-      g.a = at, g.lda = row_bytes;
-    }
-    if (b.across) {
-      if ((e = pack<BYTES>(h, b, at + bytes_a, row_bytes)) != hipSuccess) return e;
-      g.b = at + bytes_a, g.ldb = row_bytes;
-    }
+    hipError_t st = hipSuccess;
+    if (pack_a) st = pack<BYTES>(h, a, at, row_bytes);
+    if (st == hipSuccess && pack_b) st = pack<BYTES>(h, b, at + bytes_a, row_bytes);
+    if (st != hipSuccess) return st;
+    g.a = at, g.b = at + bytes_a;
   }
-  h->last_kernel = SBAMD_KERNEL_SMALL;
-  if (g.n <= 16) return launch_narrow<Tag, TOut, GATED, 1, 4>(g, h->stream);
-  if (g.n <= 32) return launch_narrow<Tag, TOut, GATED, 2, 4>(g, h->stream);
-  return launch_narrow<Tag, TOut, GATED, 4, 2>(g, h->stream);
+  g.lda = pack_a ? row_bytes : a.ld * BYTES;
+  g.ldb = pack_b ? row_bytes : b.ld * BYTES;
+  if (!pack_a) g.a = static_cast<const unsigned char*>(a.x);
+  if (!pack_b) g.b = static_cast<const unsigned char*>(b.x);
+  g.kb = pack_a && pack_b ? row_bytes : kb;  // (zeros add nothing)
+  const bool ta = pack_a || !a.across, tb = !pack_b && b.across;
+
+  h->last_kernel = family;
+  if (family == SBAMD_KERNEL_HUGE) return launch_ring_trans<Tag, TOut, GATED, 256, 256, 2, 4>(g, ta, tb, cus, h->stream);
+  if (family == SBAMD_KERNEL_LARGE) return launch_ring_trans<Tag, TOut, GATED, 128, 128, 2, 2>(g, ta, tb, cus, h->stream);
+  if (g.n <= 16) return launch_narrow<Tag, TOut, GATED, 1, 4, 2>(g, h->stream);
+  if (g.n <= 32) return launch_narrow<Tag, TOut, GATED, 2, 2, 3>(g, h->stream);
+  if (g.n <= 48) return launch_narrow<Tag, TOut, GATED, 3, 2, 2>(g, h->stream);
+  return launch_narrow<Tag, TOut, GATED, 4, 2, 2>(g, h->stream);
 }
 
 // ------------------------------------------------------------------ front ends

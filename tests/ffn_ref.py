@@ -48,6 +48,11 @@ def from_bits(s, dtype):
 
 
 def act(g, kind):
+    with np.errstate(over="ignore"):
+        return _act(g, kind)
+
+
+def _act(g, kind):
     if kind == "silu":
         return g / (1.0 + np.exp(-g))
     if kind == "gelu":

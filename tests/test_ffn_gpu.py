@@ -19,6 +19,12 @@ from common import seeded
 
 pytestmark = pytest.mark.gpu
 
+# kernels to pin: chosen by itself, narrow, 128 x 128 ring, 256 x 256 ring
+AUTO, NARROW, RING128, RING256 = (_lib.KERNEL_AUTO,), (_lib.KERNEL_SMALL,), (_lib.KERNEL_LARGE,), (_lib.KERNEL_HUGE,)
+FAMILIES = {"narrow": NARROW, "ring128": RING128, "ring256": RING256}
+# tiles whole, ragged in one or both directions, smaller than a tile; k of one step, whole steps, with a tail, shorter than a step, odd
+FAMILY_SHAPES = [(256, 256, 64), (300, 130, 96), (5, 300, 1000), (520, 70, 40), (129, 257, 31), (257, 513, 333), (64, 1, 2050), (1, 640, 192)]
+
 GUARD = 64  # elements in front of and behind every device matrix
 STORE = {"float32": np.float32, "float16": np.uint16, "bfloat16": np.uint16, "int8": np.int8}
 FILL = {"float32": np.float32(-12345.0), "float16": np.uint16(0x7BCD), "bfloat16": np.uint16(0x7BCD), "int8": np.int8(-77)}
@@ -142,7 +148,7 @@ def across(a):
     return np.ascontiguousarray(a.T)
 
 
-def run_scaled(h, out, n, m, k, ta="t", tb="n", alpha=1.0, beta=0.0, pad=0, shift=0, scales="both", family=_lib.KERNEL_AUTO):
+def run_scaled(h, out, n, m, k, ta="t", tb="n", alpha=1.0, beta=0.0, pad=0, shift=0, scales="both", family=AUTO):
     rng = seeded("scaled", out, n, m, k, ta, tb, alpha, beta, pad, shift, scales)
     x, w = int8_operands(rng, n, m, k)
     sx = np.exp(rng.standard_normal(n)).astype(np.float32) if scales != "none" else None
@@ -152,7 +158,7 @@ def run_scaled(h, out, n, m, k, ta="t", tb="n", alpha=1.0, beta=0.0, pad=0, shif
     xg = Mat(h, "int8", n, k, k + pad, shift, x) if tb == "n" else Mat(h, "int8", k, n, n + pad, shift, across(x))
     cg = Mat(h, out, n, m, m + pad, shift, c_bits)
     sxg, swg = (None if s is None else vec(h, s) for s in (sx, sw))
-    h.set_kernel(family)
+    h.set_kernel(*family)
     h.wait(sb._gemm_scaled(h, ta, tb, m, n, k, alpha, wg.buf, wg.ld, swg and swg.buf, xg.buf, xg.ld, sxg and sxg.buf, beta, cg.buf,
                            cg.ld))
     s = (x.astype(np.int64) @ w.astype(np.int64).T).astype(np.float64)
@@ -170,6 +176,14 @@ def run_scaled(h, out, n, m, k, ta="t", tb="n", alpha=1.0, beta=0.0, pad=0, shif
                                    (33, 257, 1000), (64, 16, 640), (65, 48, 1153), (130, 70, 2048), (300, 513, 333)])
 def test_scaled_sizes(h, out, n, m, k):
     run_scaled(h, out, n, m, k)
+
+
+@pytest.mark.parametrize("family", FAMILIES)
+@pytest.mark.parametrize("n,m,k", FAMILY_SHAPES)
+def test_scaled_families(h, family, n, m, k):
+    for out, pad in (("float32", 0), ("bfloat16", 16), ("float16", 5)):
+        run_scaled(h, out, n, m, k, beta=0.5 if pad else 0.0, pad=pad, family=FAMILIES[family])
+        assert h.last_kernel() == FAMILIES[family][0]
 
 
 @pytest.mark.parametrize("ta,tb", [("t", "n"), ("n", "n"), ("t", "t"), ("n", "t")])
@@ -232,7 +246,7 @@ def test_scaled_poisoned_columns_and_tiny_scales(h):
 
 
 # ---------------------------------------------------------------- gated block
-def run_gated(h, dtype, n, m, k, kind, ta="t", tb="n", keep=False, pad=0, shift=0, family=_lib.KERNEL_AUTO, size=1.0):
+def run_gated(h, dtype, n, m, k, kind, ta="t", tb="n", keep=False, pad=0, shift=0, family=AUTO, size=1.0):
     rng = seeded("gated", dtype, n, m, k, kind, ta, tb, keep, pad, shift)
     xb, x = ref.to_bits(rng.standard_normal((n, k)) * size, dtype)
     wb, w = ref.to_bits(rng.standard_normal((2 * m, k)) * (2.0 / math.sqrt(max(k, 1))), dtype)
@@ -240,7 +254,7 @@ def run_gated(h, dtype, n, m, k, kind, ta="t", tb="n", keep=False, pad=0, shift=
     xg = Mat(h, dtype, n, k, k + pad, shift, xb) if tb == "n" else Mat(h, dtype, k, n, n + pad, shift, across(xb))
     cg = Mat(h, dtype, n, m, m + pad, shift)
     pg = Mat(h, dtype, n, 2 * m, 2 * m + pad, shift) if keep else None
-    h.set_kernel(family)
+    h.set_kernel(*family)
     args = (pg.buf, pg.ld) if keep else ()
     h.wait(sb._gated_gemm(h, activation_t[kind], ta, tb, m, n, k, wg.buf, wg.ld, xg.buf, xg.ld, cg.buf, cg.ld, *args))
     p, p_err = x @ w.T, ref.product_error(x, w, k)
@@ -256,6 +270,15 @@ def run_gated(h, dtype, n, m, k, kind, ta="t", tb="n", keep=False, pad=0, shift=
                                    (48, 64, 1024), (65, 129, 77), (130, 257, 300), (256, 128, 64), (257, 130, 200)])
 def test_gated_sizes(h, dtype, n, m, k):
     run_gated(h, dtype, n, m, k, "silu", keep=(n + m) % 2 == 0)
+
+
+@pytest.mark.parametrize("family", FAMILIES)
+@pytest.mark.parametrize("n,m,k", FAMILY_SHAPES)
+@pytest.mark.parametrize("ta,tb", [("t", "n"), ("n", "n"), ("t", "t"), ("n", "t")])
+def test_gated_families(h, family, n, m, k, ta, tb):
+    """Every kernel on every layout: m a multiple of 8 or not decides whether an operand across k is read in place."""
+    for dtype, pad, keep in (("bfloat16", 0, True), ("float16", 8, False), ("bfloat16", 3, True)):
+        run_gated(h, dtype, n, m, k, "silu", ta, tb, keep, pad, family=FAMILIES[family])
 
 
 @pytest.mark.parametrize("kind", ref.ACTS)
@@ -294,7 +317,7 @@ def test_gated_keeps_nan_and_infinity_in_their_token(h, n):
         assert np.isnan(got[n - 1]).all() and np.isfinite(got[: n - 1]).all(), kind
 
 
-def run_gated_scaled(h, out, n, m, k, kind, ta="t", tb="n", pad=0, shift=0, scales=True, family=_lib.KERNEL_AUTO):
+def run_gated_scaled(h, out, n, m, k, kind, ta="t", tb="n", pad=0, shift=0, scales=True, family=AUTO):
     rng = seeded("gated scaled", out, n, m, k, kind, ta, tb, pad, shift, scales)
     x, w = int8_operands(rng, n, 2 * m, k)
     sx = (np.exp(0.5 * rng.standard_normal(n)) / 75.0).astype(np.float32)
@@ -305,7 +328,7 @@ def run_gated_scaled(h, out, n, m, k, kind, ta="t", tb="n", pad=0, shift=0, scal
     xg = Mat(h, "int8", n, k, k + pad, shift, x) if tb == "n" else Mat(h, "int8", k, n, n + pad, shift, across(x))
     cg = Mat(h, out, n, m, m + pad, shift)
     swg, sxg = vec(h, sw) if scales else None, vec(h, sx)
-    h.set_kernel(family)
+    h.set_kernel(*family)
     h.wait(sb._gated_gemm_scaled(h, activation_t[kind], ta, tb, m, n, k, wg.buf, wg.ld, swg and swg.buf, xg.buf, xg.ld, sxg.buf,
                                  cg.buf, cg.ld))
     s = (x.astype(np.int64) @ w.astype(np.int64).T).astype(np.float64)
@@ -318,6 +341,13 @@ def run_gated_scaled(h, out, n, m, k, kind, ta="t", tb="n", pad=0, shift=0, scal
 @pytest.mark.parametrize("n,m,k", [(1, 1, 3), (1, 40, 256), (16, 17, 127), (33, 64, 130), (64, 100, 1000), (130, 257, 512), (300, 70, 64)])
 def test_gated_scaled_sizes(h, out, n, m, k):
     run_gated_scaled(h, out, n, m, k, "silu")
+
+
+@pytest.mark.parametrize("family", FAMILIES)
+@pytest.mark.parametrize("n,m,k", FAMILY_SHAPES)
+def test_gated_scaled_families(h, family, n, m, k):
+    for out, pad in (("float32", 0), ("bfloat16", 16), ("float16", 5)):
+        run_gated_scaled(h, out, n, m, k, "gelu_tanh", pad=pad, family=FAMILIES[family])
 
 
 @pytest.mark.parametrize("kind", ref.ACTS)
