@@ -79,6 +79,12 @@ struct FfnArgs {
   int32_t beta_zero;
   int32_t act;
   int32_t tiles_m, tiles_n;
+  // Cut products (the gradients): the first `whole` tiles are worked through in one go, the others in `slabs` pieces of `chunk` 16-bit
+  // units of k whose float sums go to the cube, piece after piece, tile [BN tokens][BM channels].
+  int32_t whole = 0, slabs = 1;
+  int64_t chunk = 0;
+  float* cube = nullptr;
+  int64_t lim_b = 0;  // tokens of b that may be read where b lies across k and is padded behind the last one (0: n)
 };
 
 // ---------------------------------------------------------------- activations
@@ -373,6 +379,7 @@ constexpr int CORNER_ROW = 128, CORNER_BYTES = 32 * CORNER_ROW;
 __device__ inline int corner_at(int row, int byte) { return row * CORNER_ROW + (((byte >> 4) ^ ((row >> 1) & 7)) << 4) + (byte & 15); }
 
 // 32 tokens x SLAB channels of SB-byte elements (2: already of type TOut; 4: floats) from the corner to rows of `out`.
+// (One store instruction per 64 pieces, always, where `vec` and every row and channel exists: the ring counts on it.)
 template <int SB, int SLAB, typename TOut>
 __device__ inline void corner_to_rows(const SBAMD_LDS unsigned char* corner, TOut* out, int64_t ld, int64_t ch0, int64_t ch_lim, int64_t t0,
                                       int64_t t_lim, bool vec, int lane, bool read_c, float beta) {
@@ -420,7 +427,7 @@ __device__ inline void corner_to_rows(const SBAMD_LDS unsigned char* corner, TOu
   }
 }
 
-template <typename Tag, typename TOut, bool GATED, bool TA, bool TB, int BM, int BN, int WM, int WN>
+template <typename Tag, typename TOut, bool GATED, bool CUT, bool TA, bool TB, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(WM* WN * 64, 2) ffn_ring_kernel(const FfnArgs<TOut> g) {
   constexpr int NT = WM * WN * 64;
   constexpr int WTM = BM / WM, WTN = BN / WN;
@@ -442,19 +449,34 @@ __global__ void __launch_bounds__(WM* WN * 64, 2) ffn_ring_kernel(const FfnArgs<
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave % WM, wn = wave / WM;
 
-  const int64_t lda = g.lda / 2, ldb = g.ldb / 2, k_len = g.kb / 2;  // in 16-bit units
+  const int64_t lda = g.lda / 2, ldb = g.ldb / 2;  // in 16-bit units
   const int tiles = g.tiles_m * g.tiles_n;
+  const int units = CUT ? g.whole + (tiles - g.whole) * g.slabs : tiles;  // a unit of work: a tile, or a slab of one
   OpA oa;
   OpB ob;
-  int64_t m0, n0;
+  int64_t m0, n0, k_len;
   float sa[WTM / 64], sb[NI];  // scales: lane's rows lane, lane + 64 of the wavefront tile; lane's token of each 32-token block
-  auto begin = [&](int tile) {
-    int tm, tn;
-    tile_coords(xcd_remap(tile, tiles), g.tiles_m, g.tiles_n, tm, tn);
+  int piece = 0;  // CUT: which slab of the cube, counted from 0; whole tiles have none
+  auto begin = [&](int unit) {
+    const uint16_t* a = reinterpret_cast<const uint16_t*>(g.a);
+    const uint16_t* b = reinterpret_cast<const uint16_t*>(g.b);
+    int tm, tn, tile;
+    k_len = g.kb / 2;
+    if (!CUT || unit < g.whole) {
+      tile = xcd_remap(unit, CUT ? g.whole : tiles);
+    } else {
+      piece = xcd_remap(unit - g.whole, units - g.whole);
+      tile = g.whole + piece / g.slabs;
+      const int64_t k0 = int64_t(piece % g.slabs) * g.chunk;
+      k_len = k_len - k0 < g.chunk ? k_len - k0 : g.chunk;
+      a += TA ? k0 : k0 * lda;
+      b += TB ? k0 * ldb : k0;
+    }
+    tile_coords(tile, g.tiles_m, g.tiles_n, tm, tn);
     m0 = int64_t(tm) * CHB, n0 = int64_t(tn) * BN;
-    if constexpr (GATED) oa.init_gated(reinterpret_cast<const uint16_t*>(g.a), lda, m0, g.m, tid);
-    else oa.init(reinterpret_cast<const uint16_t*>(g.a), lda, m0, g.m, tid);
-    ob.init(reinterpret_cast<const uint16_t*>(g.b), ldb, n0, g.n, tid);
+    if constexpr (GATED) oa.init_gated(a, lda, m0, g.m, tid);
+    else oa.init(a, lda, m0, g.m, tid);
+    ob.init(b, ldb, n0, CUT && g.lim_b > 0 ? g.lim_b : g.n, tid);
     if constexpr (SCALED) {  // (rows and tokens past the edge read the last one: they only feed what is not stored)
 #pragma unroll
       for (int i = 0; i < WTM / 64; ++i) {
@@ -473,8 +495,11 @@ __global__ void __launch_bounds__(WM* WN * 64, 2) ffn_ring_kernel(const FfnArgs<
     ring_start<OpA, OpB, RING_STAGES>(oa, ob, lda, ldb, int(k_len / RING_BK), smem, wave);
   };
 
+  // vector stores of a whole tile's epilogue, per wavefront
+  constexpr int STORES = NI * 32 * CHW * int(sizeof(TOut)) / 1024;
+  bool stored = false;  // the last epilogue issued exactly STORES of them behind the loads of the tile to come
   begin(blockIdx.x);
-  for (int tile = blockIdx.x;;) {
+  for (int unit = blockIdx.x;;) {
     Acc acc[MI][NI];
 #pragma unroll
     for (int i = 0; i < MI; ++i)
@@ -483,10 +508,13 @@ __global__ void __launch_bounds__(WM* WN * 64, 2) ffn_ring_kernel(const FfnArgs<
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
     // (its first barrier lies behind every wavefront's epilogue of the tile before, so the last stage may be refilled)
-    ring_multiply<Tag, OpA, OpB, MI, NI, WTM, WTN, 0, false, RING_STAGES, true>(acc, oa, ob, lda, ldb, k_len, smem, tid, lane, wave, wm, wn);
+    ring_multiply<Tag, OpA, OpB, MI, NI, WTM, WTN, 0, false, RING_STAGES, true, STORES>(acc, oa, ob, lda, ldb, k_len, smem, tid, lane, wave, wm,
+                                                                                       wn, stored);
 
     __syncthreads();  // every wavefront is through with the ring's stages
     const int64_t ch0 = m0 + wm * CHW, tok0 = n0 + wn * WTN;
+    const bool partial = CUT && unit >= g.whole;
+    const int piece_now = piece;
     float sa_now[WTM / 64], sb_now[NI];
     if constexpr (SCALED) {
 #pragma unroll
@@ -494,8 +522,8 @@ __global__ void __launch_bounds__(WM* WN * 64, 2) ffn_ring_kernel(const FfnArgs<
 #pragma unroll
       for (int j = 0; j < NI; ++j) sb_now[j] = sb[j];
     }
-    const int next = tile + int(gridDim.x);
-    if (next < tiles) begin(next);
+    const int next = unit + int(gridDim.x);
+    if (next < units) begin(next);
 
     // The epilogue's addresses are made from a lane index the compiler cannot see through: it would otherwise compute them
     // all in front of the tile loop and spill them.
@@ -519,8 +547,10 @@ __global__ void __launch_bounds__(WM* WN * 64, 2) ffn_ring_kernel(const FfnArgs<
       return v;
     };
     // value(i, q) of 32-channel blocks i = B0 .. B0 + BLOCKS - 1 of the wavefront's channels, through the corner to `out`
-    auto emit = [&](auto sb_tag, auto j_tag, auto&& value, TOut* out, int64_t ld, int64_t lim, bool vec, bool read_c) {
+    auto emit_at = [&](auto sb_tag, auto j_tag, auto&& value, auto* out, int64_t ld, int64_t ch_at, int64_t ch_lim, int64_t tok_at,
+                       int64_t tok_lim, bool vec, bool read_c) {
       constexpr int SB = decltype(sb_tag)::value, J = decltype(j_tag)::value;
+      using TTo = std::remove_pointer_t<decltype(out)>;
       constexpr int SLAB = CHW * SB < CORNER_ROW ? CHW : CORNER_ROW / SB, BLOCKS = SLAB / 32;
       static_for<CHW / SLAB>([&](auto slab) {
         constexpr int B0 = decltype(slab)::value * BLOCKS;
@@ -542,9 +572,13 @@ __global__ void __launch_bounds__(WM* WN * 64, 2) ffn_ring_kernel(const FfnArgs<
           });
         });
         settle();
-        corner_to_rows<SB, SLAB, TOut>(corner, out, ld, ch0 + decltype(slab)::value * SLAB, lim, tok0 + J * 32, g.n, vec, lane_e, read_c, g.beta);
+        corner_to_rows<SB, SLAB, TTo>(corner, out, ld, ch_at + decltype(slab)::value * SLAB, ch_lim, tok_at + J * 32, tok_lim, vec, lane_e,
+                                      read_c, g.beta);
         settle();
       });
+    };
+    auto emit = [&](auto sb_tag, auto j_tag, auto&& value, TOut* out, int64_t ld, bool vec, bool read_c) {
+      emit_at(sb_tag, j_tag, value, out, ld, ch0, g.m, tok0, g.n, vec, read_c);
     };
     auto rows_aligned = [](const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (ld * int64_t(sizeof(TOut))) % 16 == 0; };
     using own_size = std::integral_constant<int, int(sizeof(TOut))>;
@@ -556,8 +590,8 @@ __global__ void __launch_bounds__(WM* WN * 64, 2) ffn_ring_kernel(const FfnArgs<
       if (g.p) {
         const bool vec_p = rows_aligned(g.p, g.ldp);
         static_for<NI>([&](auto j) {
-          emit(own_size{}, j, gate, g.p, g.ldp, g.m, vec_p, false);
-          emit(own_size{}, j, up, g.p + g.m, g.ldp, g.m, vec_p && rows_aligned(g.p + g.m, g.ldp), false);
+          emit(own_size{}, j, gate, g.p, g.ldp, vec_p, false);
+          emit(own_size{}, j, up, g.p + g.m, g.ldp, vec_p && rows_aligned(g.p + g.m, g.ldp), false);
         });
       }
       with_act(g.act, [&](auto act) {
@@ -568,7 +602,7 @@ __global__ void __launch_bounds__(WM* WN * 64, 2) ffn_ring_kernel(const FfnArgs<
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = act_value<decltype(act)::value>(x[e]) * y[e];
             return v;
-          }, g.c, g.ldc, g.m, vec_c, false);
+          }, g.c, g.ldc, vec_c, false);
         });
       });
     } else {
@@ -578,14 +612,59 @@ __global__ void __launch_bounds__(WM* WN * 64, 2) ffn_ring_kernel(const FfnArgs<
         for (int e = 0; e < 4; ++e) v[e] = g.alpha * v[e];
         return v;
       };
-      static_for<NI>([&](auto j) {
-        if (g.beta_zero) emit(own_size{}, j, scaled, g.c, g.ldc, g.m, vec_c, false);
-        else emit(as_float{}, j, scaled, g.c, g.ldc, g.m, vec_c, true);
-      });
+      if (partial) {
+        float* tile_sums = g.cube + int64_t(piece_now) * (BM * BN);
+        static_for<NI>([&](auto j) { emit_at(as_float{}, j, scaled, tile_sums, BM, wm * CHW, BM, wn * WTN, BN, true, false); });
+      } else if (g.beta_zero) {
+        static_for<NI>([&](auto j) { emit(own_size{}, j, scaled, g.c, g.ldc, vec_c, false); });
+      } else {
+        static_for<NI>([&](auto j) { emit(as_float{}, j, scaled, g.c, g.ldc, vec_c, true); });
+      }
     }
-    if (next >= tiles) return;
-    tile = next;
+    // (with P kept there are more stores than that: waiting for fewer is then merely early)
+    stored = vec_c && !partial && (GATED || g.beta_zero) && ch0 + CHW <= g.m && tok0 + WTN <= g.n;
+    if (next >= units) return;
+    unit = next;
   }
+}
+
+// The cut tiles: slabs added in order, then beta * C, rounded once.  Eight channels of one token per thread.
+template <typename TOut, int BM, int BN>
+__global__ void __launch_bounds__(256) ffn_join_kernel(const FfnArgs<TOut> g) {
+  const int64_t v = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  constexpr int PER_TILE = BM * BN / 8;
+  const int t = int(v / PER_TILE), at = int(v % PER_TILE) * 8;  // (the grid is whole tiles)
+  int tm, tn;
+  tile_coords(g.whole + t, g.tiles_m, g.tiles_n, tm, tn);
+  const int64_t ch = int64_t(tm) * BM + at % BM, tok = int64_t(tn) * BN + at / BM;
+  if (ch >= g.m || tok >= g.n) return;
+  const float* src = g.cube + int64_t(t) * g.slabs * (BM * BN) + at;
+  f32x4_t lo = *reinterpret_cast<const f32x4_t*>(src), hi = *reinterpret_cast<const f32x4_t*>(src + 4);
+  for (int s = 1; s < g.slabs; ++s) {
+    src += BM * BN;
+    lo += *reinterpret_cast<const f32x4_t*>(src);
+    hi += *reinterpret_cast<const f32x4_t*>(src + 4);
+  }
+  TOut* out = g.c + ch + tok * g.ldc;
+  const bool vec = ch + 8 <= g.m && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  union {
+    TOut e[8];
+    i32x4 q;
+  } x;
+  static_assert(sizeof(TOut) == 2, "16-bit results");
+  if (vec && !g.beta_zero) x.q = *reinterpret_cast<const i32x4*>(out);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float f = e < 4 ? lo[e & 3] : hi[e & 3];
+    if (vec) {
+      if (!g.beta_zero) f = f + g.beta * load_out(&x.e[e]);
+      store_out(&x.e[e], f);
+    } else if (ch + e < g.m) {
+      if (!g.beta_zero) f = f + g.beta * load_out(out + e);
+      store_out(out + e, f);
+    }
+  }
+  if (vec) *reinterpret_cast<i32x4*>(out) = x.q;
 }
 
 // -------------------------------------------------------------------- repack

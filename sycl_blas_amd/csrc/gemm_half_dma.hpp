@@ -205,11 +205,13 @@ struct RingOperand {
 // instructions, bit 4: no fragment reads); the library instantiates 0.
 // acc += (the tile of op(A)) * (the tile of op(B)) over k_len, the operands' pointers set up by init: the ring itself.
 // M_FIRST: a lane ends up with one index of A (lane & 31) and sixteen of B, else the other way round.
-// STAGES - 1 tiles are kept in flight.  STARTED: the first ones are on their way already (ring_start).
-template <typename Tag, typename OpA, typename OpB, int MI, int NI, int WTM, int WTN, int ABLATE, bool M_FIRST, int STAGES, bool STARTED, typename Acc>
+// STAGES - 1 tiles are kept in flight.  STARTED: the first ones are on their way already (ring_start), and `stores` says that
+// exactly STORES vector stores (and nothing else) were issued behind them: memory operations complete in order, so the first
+// tiles are waited for without waiting for those stores.
+template <typename Tag, typename OpA, typename OpB, int MI, int NI, int WTM, int WTN, int ABLATE, bool M_FIRST, int STAGES, bool STARTED, int STORES = 0, typename Acc>
 __device__ __attribute__((always_inline)) inline void ring_multiply(Acc (&acc)[MI][NI], OpA& oa, OpB& ob, const int64_t lda, const int64_t ldb,
                                                                     const int64_t k_len, SBAMD_LDS unsigned char* smem, const int tid,
-                                                                    const int lane, const int wave, const int wm, const int wn) {
+                                                                    const int lane, const int wave, const int wm, const int wn, const bool stores = false) {
   constexpr int NM = MI * NI;   // matrix instructions per half step
   constexpr int NPA = OpA::NP, NPB = OpB::NP;    // load instructions per thread and tile of each operand
   constexpr int LPA = NPA / 2, LPH = LPA + NPB / 2;  // of them per half step: A's, both operands'
@@ -234,7 +236,9 @@ __device__ __attribute__((always_inline)) inline void ring_multiply(Acc (&acc)[M
     }
   }
   // tile 0 must have landed for every wave before anyone reads it (the tiles behind it may be in flight)
-  if (nk > AHEAD - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((AHEAD - 1) * (NPA + NPB)) : "memory");
+  static_assert((AHEAD - 1) * (NPA + NPB) + STORES < 64, "the counter's range");
+  if (STORES > 0 && stores && nk > AHEAD - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((AHEAD - 1) * (NPA + NPB) + STORES) : "memory");
+  else if (nk > AHEAD - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((AHEAD - 1) * (NPA + NPB)) : "memory");
   else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
 
@@ -289,8 +293,9 @@ __device__ __attribute__((always_inline)) inline void ring_multiply(Acc (&acc)[M
   // One K step.  LOADS: tile t + AHEAD exists and is issued here; NEXT: tile
   // t + 1 exists.
   auto step = [&](const SBAMD_LDS unsigned char* cur, const SBAMD_LDS unsigned char* next, SBAMD_LDS unsigned char* fill,
-                  auto loads_tag, auto next_tag) {
+                  auto loads_tag, auto next_tag, auto extra_tag) {
     constexpr bool LOADS = decltype(loads_tag)::value;
+    constexpr int EXTRA = decltype(extra_tag)::value;  // stores that may still be out as well
 
     // the fragments fetched during the previous half step must have arrived (the
     // transposing reads are inline assembly: the compiler does not wait for them)
@@ -303,7 +308,7 @@ __device__ __attribute__((always_inline)) inline void ring_multiply(Acc (&acc)[M
 
     // every fragment read of tile t has returned; own pieces of tile t + 1 have landed
     // (in flight and allowed to stay so: tiles t + 2 .. t + AHEAD - 1 and the first half of tile t + AHEAD)
-    if (LOADS && !(ABLATE & 1)) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((AHEAD - 2) * (NPA + NPB) + LPH) : "memory");
+    if (LOADS && !(ABLATE & 1)) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((AHEAD - 2) * (NPA + NPB) + LPH + EXTRA) : "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
@@ -322,17 +327,29 @@ __device__ __attribute__((always_inline)) inline void ring_multiply(Acc (&acc)[M
   // Steady state: as many steps per trip as there are stages, so that every LDS address is the lane's offset plus a
   // compile-time constant.
   int t = 0;
+  using none = std::integral_constant<int, 0>;
+  if constexpr (STORES > 0) {
+    // the tiles that were in flight before the stores: AHEAD - 1 of them are waited for in steps 0 .. AHEAD - 2
+    if (stores && t + STAGES - 1 + AHEAD < nk) {
+      static_for<STAGES>([&](auto i_tag) {
+        constexpr int I = decltype(i_tag)::value;
+        step(smem + I * RING_STAGE_BYTES, smem + (I + 1) % STAGES * RING_STAGE_BYTES, smem + (I + STAGES - 1) % STAGES * RING_STAGE_BYTES,
+             yes{}, yes{}, std::integral_constant<int, (I < AHEAD - 1 ? STORES : 0)>{});
+      });
+      t = STAGES;
+    }
+  }
   for (; t + STAGES - 1 + AHEAD < nk; t += STAGES) {
     static_for<STAGES>([&](auto i_tag) {
       constexpr int I = decltype(i_tag)::value;
       step(smem + I * RING_STAGE_BYTES, smem + (I + 1) % STAGES * RING_STAGE_BYTES, smem + (I + STAGES - 1) % STAGES * RING_STAGE_BYTES, yes{},
-           yes{});
+           yes{}, none{});
     });
   }
   // the remaining steps (t is a multiple of STAGES here) with the stage computed at run time
-  for (; t + AHEAD < nk; ++t) step(stage_ptr(t), stage_ptr(t + 1), stage_ptr(t + AHEAD), yes{}, yes{});
-  for (; t + 1 < nk; ++t) step(stage_ptr(t), stage_ptr(t + 1), stage_ptr(t + AHEAD), no{}, yes{});
-  if (t < nk) step(stage_ptr(t), stage_ptr(t + 1), stage_ptr(t + AHEAD), no{}, no{});
+  for (; t + AHEAD < nk; ++t) step(stage_ptr(t), stage_ptr(t + 1), stage_ptr(t + AHEAD), yes{}, yes{}, none{});
+  for (; t + 1 < nk; ++t) step(stage_ptr(t), stage_ptr(t + 1), stage_ptr(t + AHEAD), no{}, yes{}, none{});
+  if (t < nk) step(stage_ptr(t), stage_ptr(t + 1), stage_ptr(t + AHEAD), no{}, no{}, none{});
 
   // K tail (k % 32 valid k): one more tile, zero-padded, staged through registers into stage 0 once every
   // wavefront has finished the last ring step; the zeros add nothing to the sums.

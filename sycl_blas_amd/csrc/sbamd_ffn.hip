@@ -63,9 +63,9 @@ hipError_t pack(Handle* h, const Rows& o, unsigned char* dst, int64_t row_bytes)
   return hipGetLastError();
 }
 
-template <typename Tag, typename TOut, bool GATED, bool TA, bool TB, int BM, int BN, int WM, int WN>
+template <typename Tag, typename TOut, bool GATED, bool CUT, bool TA, bool TB, int BM, int BN, int WM, int WN>
 hipError_t launch_ring(FfnArgs<TOut> g, int cus, hipStream_t stream) {
-  auto kernel = ffn_ring_kernel<Tag, TOut, GATED, TA, TB, BM, BN, WM, WN>;
+  auto kernel = ffn_ring_kernel<Tag, TOut, GATED, CUT, TA, TB, BM, BN, WM, WN>;
   constexpr int lds = ring_lds_bytes(BM, BN);
   static PerDeviceOnce lds_limit;
   const hipError_t e = lds_limit.run([&] {
@@ -77,19 +77,20 @@ hipError_t launch_ring(FfnArgs<TOut> g, int cus, hipStream_t stream) {
   if (tm > 0x7fff0000LL / tn) return hipErrorInvalidValue;
   g.tiles_m = int32_t(tm);
   g.tiles_n = int32_t(tn);
-  const int64_t resident = int64_t(cus) * (160 * 1024 / lds);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(tm * tn, resident)), dim3(WM * WN * 64), lds, stream, g);
+  const int64_t resident = int64_t(cus) * (160 * 1024 / lds), units = CUT ? g.whole + (tm * tn - g.whole) * g.slabs : tm * tn;
+  if (units > 0x7fff0000LL) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(units, resident)), dim3(WM * WN * 64), lds, stream, g);
   return hipGetLastError();
 }
 
-template <typename Tag, typename TOut, bool GATED, int BM, int BN, int WM, int WN>
+template <typename Tag, typename TOut, bool GATED, bool CUT, int BM, int BN, int WM, int WN>
 hipError_t launch_ring_trans(const FfnArgs<TOut>& g, bool ta, bool tb, int cus, hipStream_t stream) {
   // 8-bit operands always lie along k here: the transposing LDS reads the other layouts need move 16-bit elements
   if constexpr (std::is_same<Tag, I8Tag>::value) {
-    return launch_ring<Tag, TOut, GATED, true, false, BM, BN, WM, WN>(g, cus, stream);
+    return launch_ring<Tag, TOut, GATED, CUT, true, false, BM, BN, WM, WN>(g, cus, stream);
   } else {
-    if (ta) return tb ? launch_ring<Tag, TOut, GATED, true, true, BM, BN, WM, WN>(g, cus, stream) : launch_ring<Tag, TOut, GATED, true, false, BM, BN, WM, WN>(g, cus, stream);
-    return tb ? launch_ring<Tag, TOut, GATED, false, true, BM, BN, WM, WN>(g, cus, stream) : launch_ring<Tag, TOut, GATED, false, false, BM, BN, WM, WN>(g, cus, stream);
+    if (ta) return tb ? launch_ring<Tag, TOut, GATED, CUT, true, true, BM, BN, WM, WN>(g, cus, stream) : launch_ring<Tag, TOut, GATED, CUT, true, false, BM, BN, WM, WN>(g, cus, stream);
+    return tb ? launch_ring<Tag, TOut, GATED, CUT, false, true, BM, BN, WM, WN>(g, cus, stream) : launch_ring<Tag, TOut, GATED, CUT, false, false, BM, BN, WM, WN>(g, cus, stream);
   }
 }
 
@@ -164,8 +165,8 @@ hipError_t run_ffn(Handle* h, const Rows& a, const Rows& b, FfnArgs<TOut> g) {
   const bool ta = pack_a || !a.across, tb = !pack_b && b.across;
 
   h->last_kernel = family;
-  if (family == SBAMD_KERNEL_HUGE) return launch_ring_trans<Tag, TOut, GATED, 256, 256, 2, 4>(g, ta, tb, cus, h->stream);
-  if (family == SBAMD_KERNEL_LARGE) return launch_ring_trans<Tag, TOut, GATED, 128, 128, 2, 2>(g, ta, tb, cus, h->stream);
+  if (family == SBAMD_KERNEL_HUGE) return launch_ring_trans<Tag, TOut, GATED, false, 256, 256, 2, 4>(g, ta, tb, cus, h->stream);
+  if (family == SBAMD_KERNEL_LARGE) return launch_ring_trans<Tag, TOut, GATED, false, 128, 128, 2, 2>(g, ta, tb, cus, h->stream);
   if (g.n <= 16) return launch_narrow<Tag, TOut, GATED, 1, 4, 2>(g, h->stream);
   if (g.n <= 32) return launch_narrow<Tag, TOut, GATED, 2, 2, 3>(g, h->stream);
   if (g.n <= 48) return launch_narrow<Tag, TOut, GATED, 3, 2, 2>(g, h->stream);
@@ -274,19 +275,96 @@ int quantize(sbamd_handle_t hh, int64_t m, int64_t n, const typename QuantIn<Tag
   return e == hipSuccess ? SBAMD_OK : ffn_fail(h, e, "quantise launch");
 }
 
-// C of type TOut = alpha op(A) op(B) + beta C on the 16-bit GEMM back end, single product.
+// C = op(A) op(B) + beta C in 16 bits, C rounded once: the gradients' products.
 template <typename TOut>
-Problem<uint16_t, TOut> product(bool ta, bool tb, int64_t m, int64_t n, int64_t k, const uint16_t* a, int64_t lda, const uint16_t* b,
-                                int64_t ldb, float beta, TOut* c, int64_t ldc) {
-  Problem<uint16_t, TOut> q{};
-  q.ta = ta, q.tb = tb, q.m = m, q.n = n, q.k = k;
-  q.a = a, q.lda = lda, q.b = b, q.ldb = ldb, q.c = c, q.ldc = ldc;
-  q.batch = 1;
-  q.beta_zero = beta == 0.0f;
-  return q;
+struct Product {
+  bool ta, tb;
+  int64_t m, n, k;
+  const uint16_t* a;
+  int64_t lda;
+  const uint16_t* b;
+  int64_t ldb;
+  float beta;
+  TOut* c;
+  int64_t ldc;
+  int64_t lim_b;  // see FfnArgs
+};
+
+// How the ring works through `tiles` tiles of EDGE x EDGE: the first `whole` in one go, the rest in `slabs` pieces along k.
+struct RingPlan {
+  double time;
+  int32_t whole, slabs;
+  int64_t chunk;
+};
+// Estimated microseconds as in pick_ffn; a tile count that leaves the last round of units mostly idle (128 or 336 tiles of
+// 256 x 256 on 256 units) has that round's tiles cut along k into as many pieces as fill it, at the price of the pieces' float sums
+// going out and coming back (4.5 TB/s) and a second launch.
+template <int EDGE>
+RingPlan plan_ring(int64_t m, int64_t n, int64_t k, int cus) {
+  const int64_t tiles = ceil_div(m, EDGE) * ceil_div(n, EDGE);
+  const double len = 2.0 * double(k), per_tile = EDGE == 256 ? 6.0 : 0.7, per_byte = EDGE == 256 ? 13e-3 : 5.5e-3;
+  auto round_of = [&](double share, double bytes) {  // one round with `share` of the units busy
+    return EDGE == 256 ? 6.0 + bytes * (8.2e-3 + 4.5e-3 * share) : 0.7 + bytes * (3.3e-3 + 2.6e-3 * share);
+  };
+  const int64_t rounds = tiles / cus, rest = tiles - rounds * cus;
+  const double t_whole = 3.0 + double(rounds) * (per_tile + len * per_byte);
+  RingPlan best = {t_whole + (rest ? round_of(double(rest) / cus, len) : 0.0), int32_t(std::min<int64_t>(tiles, 0x7fff0000LL)), 1, k};
+  if (rest == 0 || tiles > 0x7fff0000LL) return best;
+  for (int64_t s = 2; s <= 32 && s * rest <= cus; ++s) {
+    const int64_t chunk = RING_BK * ceil_div(k, RING_BK * s), slabs = ceil_div(k, chunk);
+    if (slabs < 2 || chunk < 8 * RING_BK) continue;
+    const double cube = double(rest) * double(slabs) * EDGE * EDGE * 4.0;
+    const double t = t_whole + round_of(double(rest * slabs) / cus, 2.0 * double(chunk)) + 4.0 + 2.0 * cube / 4.5e6;
+    if (t < best.time) best = {t, int32_t(rounds * cus), int32_t(slabs), chunk};
+  }
+  return best;
 }
-hipError_t run_product(Handle* h, const Problem<uint16_t, uint16_t>& q, float beta) { return run_gemm_h(h, q, 1.0f, beta); }
-hipError_t run_product(Handle* h, const Problem<uint16_t, bf16_bits>& q, float beta) { return run_gemm_b(h, q, 1.0f, beta); }
+
+template <typename Tag, typename TOut, int EDGE, int WM, int WN>
+hipError_t run_ring_product(Handle* h, const Product<TOut>& q, const RingPlan& plan, int cus) {
+  FfnArgs<TOut> g{};
+  g.a = reinterpret_cast<const unsigned char*>(q.a), g.lda = q.lda * 2;
+  g.b = reinterpret_cast<const unsigned char*>(q.b), g.ldb = q.ldb * 2;
+  g.m = q.m, g.n = q.n, g.kb = q.k * 2;
+  g.c = q.c, g.ldc = q.ldc;
+  g.alpha = 1.0f, g.beta = q.beta, g.beta_zero = q.beta == 0.0f ? 1 : 0;
+  g.whole = plan.whole, g.slabs = plan.slabs, g.chunk = plan.chunk;
+  g.lim_b = q.lim_b;
+  const int64_t tm = ceil_div(q.m, EDGE), tn = ceil_div(q.n, EDGE), cut = tm * tn - plan.whole;
+  hipError_t e = hipSuccess;
+  if (cut > 0) {
+    if ((e = ensure_scratch(h, size_t(cut) * size_t(plan.slabs) * EDGE * EDGE * sizeof(float))) != hipSuccess) return e;
+    g.cube = static_cast<float*>(h->scratch);
+  }
+  e = launch_ring_trans<Tag, TOut, false, true, EDGE, EDGE, WM, WN>(g, q.ta, q.tb, cus, h->stream);
+  if (e != hipSuccess || cut <= 0) return e;
+  g.tiles_m = int32_t(tm), g.tiles_n = int32_t(tn);
+  hipLaunchKernelGGL((ffn_join_kernel<TOut, EDGE, EDGE>), dim3((unsigned)(cut * (EDGE * EDGE / 8 / 256))), dim3(256), 0, h->stream, g);
+  return hipGetLastError();
+}
+
+hipError_t run_product16(Handle* h, const Problem<uint16_t, uint16_t>& p, float beta) { return run_gemm_h(h, p, 1.0f, beta); }
+hipError_t run_product16(Handle* h, const Problem<uint16_t, bf16_bits>& p, float beta) { return run_gemm_b(h, p, 1.0f, beta); }
+
+template <typename Tag, typename TOut>
+hipError_t run_product(Handle* h, const Product<TOut>& q) {
+  const int cus = h->compute_units > 0 ? h->compute_units : 256;
+  const int64_t lim_b = q.lim_b > 0 ? q.lim_b : q.n;
+  const bool ring = aligned16(q.a, q.lda * 2) && aligned16(q.b, q.ldb * 2) && q.k >= RING_BK && (q.ta || q.m % 8 == 0) && (!q.tb || lim_b % 8 == 0);
+  if (ring && h->kernel_override != SBAMD_KERNEL_SMALL) {
+    const RingPlan big = plan_ring<256>(q.m, q.n, q.k, cus), small = plan_ring<128>(q.m, q.n, q.k, cus);
+    const bool take_big = h->kernel_override == SBAMD_KERNEL_HUGE || (h->kernel_override != SBAMD_KERNEL_LARGE && big.time < small.time);
+    h->last_kernel = take_big ? SBAMD_KERNEL_HUGE : SBAMD_KERNEL_LARGE;
+    return take_big ? run_ring_product<Tag, TOut, 256, 2, 4>(h, q, big, cus) : run_ring_product<Tag, TOut, 128, 2, 2>(h, q, small, cus);
+  }
+  // operands the ring cannot read as they lie: the 16-bit GEMM back end
+  Problem<uint16_t, TOut> p{};
+  p.ta = q.ta, p.tb = q.tb, p.m = q.m, p.n = q.n, p.k = q.k;
+  p.a = q.a, p.lda = q.lda, p.b = q.b, p.ldb = q.ldb, p.c = q.c, p.ldc = q.ldc;
+  p.batch = 1;
+  p.beta_zero = q.beta == 0.0f;
+  return run_product16(h, p, q.beta);
+}
 
 template <typename Tag, typename TOut>
 int gradient(sbamd_handle_t hh, int act, char transa, char transb, int64_t m, int64_t n, int64_t k, const uint16_t* a, int64_t lda,
@@ -318,16 +396,16 @@ int gradient(sbamd_handle_t hh, int act, char transa, char transb, int64_t m, in
     if (e != hipSuccess) return ffn_fail(h, e, "gradient launch");
   }
   // The products run with n (m) == 0 too: a sum over nothing is beta times what was there.
+  TOut* out_a = reinterpret_cast<TOut*>(da);
+  TOut* out_b = reinterpret_cast<TOut*>(db);
   if (da && m > 0 && k > 0) {
-    TOut* out = reinterpret_cast<TOut*>(da);
-    const hipError_t e = ta ? run_product(h, product<TOut>(tb, true, k, 2 * m, n, b, ldb, dp, lddp, beta_a, out, ldda), beta_a)
-                            : run_product(h, product<TOut>(false, !tb, 2 * m, k, n, dp, lddp, b, ldb, beta_a, out, ldda), beta_a);
+    const hipError_t e = ta ? run_product<Tag, TOut>(h, {bool(tb), true, k, 2 * m, n, b, ldb, dp, lddp, beta_a, out_a, ldda, 0})
+                            : run_product<Tag, TOut>(h, {false, !tb, 2 * m, k, n, dp, lddp, b, ldb, beta_a, out_a, ldda, 0});
     if (e != hipSuccess) return ffn_fail(h, e, "gradient product");
   }
   if (db && n > 0 && k > 0) {
-    TOut* out = reinterpret_cast<TOut*>(db);
-    const hipError_t e = tb ? run_product(h, product<TOut>(true, ta, n, k, 2 * m, dp, lddp, a, lda, beta_b, out, lddb), beta_b)
-                            : run_product(h, product<TOut>(!ta, false, k, n, 2 * m, a, lda, dp, lddp, beta_b, out, lddb), beta_b);
+    const hipError_t e = tb ? run_product<Tag, TOut>(h, {true, bool(ta), n, k, 2 * m, dp, lddp, a, lda, beta_b, out_b, lddb, 0})
+                            : run_product<Tag, TOut>(h, {!ta, false, k, n, 2 * m, a, lda, dp, lddp, beta_b, out_b, lddb, 0});
     if (e != hipSuccess) return ffn_fail(h, e, "gradient product");
   }
   return SBAMD_OK;

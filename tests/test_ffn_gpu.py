@@ -363,7 +363,7 @@ def test_gated_scaled_layouts(h, ta, tb, n, m, k, pad, shift):
 
 
 # ------------------------------------------------------------------- gradient
-def run_grad(h, dtype, n, m, k, kind, ta="t", tb="n", pad=0, shift=0, beta_a=0.0, beta_b=0.0, in_place=False, want="ab"):
+def run_grad(h, dtype, n, m, k, kind, ta="t", tb="n", pad=0, shift=0, beta_a=0.0, beta_b=0.0, in_place=False, want="ab", family=AUTO):
     rng = seeded("grad", dtype, n, m, k, kind, ta, tb, pad, shift, beta_a, beta_b, in_place, want)
     xb, x = ref.to_bits(rng.standard_normal((n, k)), dtype)
     wb, w = ref.to_bits(rng.standard_normal((2 * m, k)) / math.sqrt(max(k, 1)), dtype)
@@ -384,6 +384,7 @@ def run_grad(h, dtype, n, m, k, kind, ta="t", tb="n", pad=0, shift=0, beta_a=0.0
     dpg = pg if in_place else Mat(h, dtype, n, 2 * m, 2 * m + 2 * pad, shift)
     dag = weights(daw) if "a" in want else None
     dbg = tokens(dbx) if "b" in want else None
+    h.set_kernel(*family)
     h.wait(sb._gated_gemm_grad(h, activation_t[kind], ta, tb, m, n, k, wg.buf if dbg else None, wg.ld, xg.buf if dag else None, xg.ld,
                                pg.buf, pg.ld, dcg.buf, dcg.ld, dpg.buf, dpg.ld, beta_a, dag and dag.buf, wg.ld, beta_b,
                                dbg and dbg.buf, xg.ld))
@@ -430,6 +431,16 @@ def test_grad_activations(h, dtype, kind):
 @pytest.mark.parametrize("pad,shift", [(0, 0), (8, 0), (3, 1)])
 def test_grad_layouts(h, ta, tb, pad, shift):
     run_grad(h, "bfloat16", 72, 40, 56, "gelu", ta, tb, pad, shift, in_place=pad == 0)
+
+
+@pytest.mark.parametrize("family", FAMILIES)
+@pytest.mark.parametrize("ta,tb", [("t", "n"), ("n", "n"), ("t", "t"), ("n", "t")])
+@pytest.mark.parametrize("n,m,k", [(256, 128, 256), (1104, 304, 136), (72, 700, 264), (600, 36, 48), (2500, 20, 40)])
+def test_grad_families(h, family, n, m, k, ta, tb):
+    """Products on every kernel, with their sums cut along the long side (1104 tokens, 1400 rows of P) and not; 36 and 20
+    channels and 2500 tokens leave rows that do not come in whole 16-byte pieces."""
+    run_grad(h, "bfloat16", n, m, k, "silu", ta, tb, beta_a=0.5 if m > 100 else 0.0, family=FAMILIES[family])
+    run_grad(h, "float16", n, m, k, "gelu_tanh", ta, tb, pad=8, beta_b=1.0 if m > 100 else 0.0, family=FAMILIES[family])
 
 
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
@@ -516,6 +527,28 @@ def test_gradient_against_differences(h, kind):
             # central differences: a third derivative of at most about 1e3 here times step^2, and cancellation of the loss
             slack = 1e3 * step ** 2 * np.abs(v).sum() ** 3 + 1e-15 * 1e3 / step
             assert abs((grad * v).sum() - (hi - lo) / (2 * step)) <= (bound * np.abs(v)).sum() + slack, (kind, name)
+
+
+@pytest.mark.parametrize("m", [2048, 4096 + 128])
+def test_ring_walks_many_tiles(h, m):
+    """More tiles than workgroups: every workgroup goes through several, the last ones ragged, with results and P leaving
+    while the next tile's operands come in.  Sampled tokens against the 64-bit form."""
+    n, k, dtype = 2600, 192, "bfloat16"
+    rng = seeded("many tiles", m)
+    xb, x = ref.to_bits(rng.standard_normal((n, k)), dtype)
+    wb, w = ref.to_bits(rng.standard_normal((2 * m, k)) / math.sqrt(k), dtype)
+    xg, wg, cg, pg = Mat(h, dtype, n, k, values=xb), Mat(h, dtype, 2 * m, k, values=wb), Mat(h, dtype, n, m), Mat(h, dtype, n, 2 * m)
+    for family in (RING128, RING256):
+        for keep in (False, True):
+            h.set_kernel(*family)
+            args = (pg.buf, 2 * m) if keep else ()
+            h.wait(sb._gated_gemm(h, activation_t.silu, "t", "n", m, n, k, wg.buf, k, xg.buf, k, cg.buf, m, *args))
+            rows = np.unique(np.concatenate([rng.integers(0, n, 200), [0, 255, 256, n - 1]]))
+            p, p_err = x[rows] @ w.T, ref.product_error(x[rows], w, k)
+            truth, bound = ref.gated(p, p_err, m, "silu", dtype)
+            close(ref.from_bits(cg.get()[rows], dtype), truth, bound, f"many tiles {family} {keep}")
+            if keep:
+                close(ref.from_bits(pg.get()[rows], dtype), p, ref.rounded(p, p_err, dtype), f"many tiles P {family}")
 
 
 # ------------------------------------------------------ offsets beyond 32 bits
