@@ -79,11 +79,11 @@ struct FfnArgs {
   int32_t beta_zero;
   int32_t act;
   int32_t tiles_m, tiles_n;
-  // Cut products (the gradients): the first `whole` tiles are worked through in one go, the others in `slabs` pieces of `chunk` 16-bit
-  // units of k whose float sums go to the cube, piece after piece, tile [BN tokens][BM channels].
+  // Cut products (not the gated block): the first `whole` tiles are worked through in one go, the others in `slabs` pieces of
+  // `chunk` 16-bit units of k whose sums (float, or integer) go to the cube, piece after piece, tile [BN tokens][BM channels].
   int32_t whole = 0, slabs = 1;
   int64_t chunk = 0;
-  float* cube = nullptr;
+  void* cube = nullptr;
   int64_t lim_b = 0;  // tokens of b that may be read where b lies across k and is padded behind the last one (0: n)
 };
 
@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(NARROW_WAVES * 64, OCC) ffn_narrow_kernel(cons
   }
   // the last, partial chunk: zeros behind the end of k (the rows' ends are not read past)
   const int rest = int(g.kb - whole * NARROW_CHUNK);
-  if (rest > 0 && wave == W - 1) {
+  if (rest > 0 && wave == 0) {  // (no wavefront has fewer whole ones)
     const int have = rest - piece * 16;  // bytes of this lane's piece that exist
     const bool long_row = g.kb >= 16;
 #pragma unroll
@@ -412,22 +412,34 @@ __device__ inline void corner_to_rows(const SBAMD_LDS unsigned char* corner, TOu
       }
     }
   } else {
-    const int ch = lane % SLAB;
-    if (ch0 + ch >= ch_lim) return;
-    for (int row = lane / SLAB; row < 32 && t0 + row < t_lim; row += 64 / SLAB) {
-      TOut* at = out + ch0 + ch + (t0 + row) * ld;
-      if constexpr (SB == 2) {
-        *reinterpret_cast<uint16_t*>(at) = *reinterpret_cast<const SBAMD_LDS uint16_t*>(corner + corner_at(row, ch * 2));
-      } else {
-        float v = *reinterpret_cast<const SBAMD_LDS float*>(corner + corner_at(row, ch * 4));
-        if (read_c) v = v + beta * load_out(at);
-        store_out(at, v);
+    // one element per lane, a whole slab of a row (or two) per instruction; eight reads ahead of their stores
+    constexpr int AT_ONCE = 64 / SLAB, STEPS = 32 / AT_ONCE, BATCH = 8;
+    const int ch = lane % SLAB, row0 = lane / SLAB;
+    const bool live = ch0 + ch < ch_lim;
+    typedef typename std::conditional<SB == 2, uint16_t, float>::type staged_t;
+#pragma unroll 1
+    for (int r = 0; r < STEPS; r += BATCH) {
+      staged_t v[BATCH];
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) v[i] = *reinterpret_cast<const SBAMD_LDS staged_t*>(corner + corner_at((r + i) * AT_ONCE + row0, ch * SB));
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const int row = (r + i) * AT_ONCE + row0;
+        if (!live || t0 + row >= t_lim) continue;
+        TOut* at = out + ch0 + ch + (t0 + row) * ld;
+        if constexpr (SB == 2) {
+          *reinterpret_cast<uint16_t*>(at) = v[i];
+        } else {
+          float f = v[i];
+          if (read_c) f = f + beta * load_out(at);
+          store_out(at, f);
+        }
       }
     }
   }
 }
 
-template <typename Tag, typename TOut, bool GATED, bool CUT, bool TA, bool TB, int BM, int BN, int WM, int WN>
+template <typename Tag, typename TOut, bool GATED, bool TA, bool TB, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(WM* WN * 64, 2) ffn_ring_kernel(const FfnArgs<TOut> g) {
   constexpr int NT = WM * WN * 64;
   constexpr int WTM = BM / WM, WTN = BN / WN;
@@ -435,6 +447,7 @@ __global__ void __launch_bounds__(WM* WN * 64, 2) ffn_ring_kernel(const FfnArgs<
   constexpr int CHW = GATED ? WTM / 2 : WTM;  // channels of C per wavefront tile
   constexpr int CHB = GATED ? BM / 2 : BM;    // and per workgroup
   constexpr bool SCALED = std::is_same<Tag, I8Tag>::value;
+  constexpr bool CUT = !GATED;  // tiles may be cut along k
   using OpA = RingOperand<TA, BM, NT>;
   using OpB = RingOperand<!TB, BN, NT>;
   using Acc = typename std::conditional<SCALED, i32x16, f32x16>::type;
@@ -613,8 +626,17 @@ __global__ void __launch_bounds__(WM* WN * 64, 2) ffn_ring_kernel(const FfnArgs<
         return v;
       };
       if (partial) {
-        float* tile_sums = g.cube + int64_t(piece_now) * (BM * BN);
-        static_for<NI>([&](auto j) { emit_at(as_float{}, j, scaled, tile_sums, BM, wm * CHW, BM, wn * WTN, BN, true, false); });
+        float* tile_sums = static_cast<float*>(g.cube) + int64_t(piece_now) * (BM * BN);
+        auto sums = [&](auto i, auto j, auto q) {  // as they are (an integer's bits merely travel as a float's)
+          f32x4_t v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const typename FfnMma<Tag>::sum_t sum = acc[decltype(i)::value][decltype(j)::value][decltype(q)::value * 4 + e];
+            v[e] = __builtin_bit_cast(float, sum);  // (of a vector's element directly it takes element 0)
+          }
+          return v;
+        };
+        static_for<NI>([&](auto j) { emit_at(as_float{}, j, sums, tile_sums, BM, wm * CHW, BM, wn * WTN, BN, true, false); });
       } else if (g.beta_zero) {
         static_for<NI>([&](auto j) { emit(own_size{}, j, scaled, g.c, g.ldc, vec_c, false); });
       } else {
@@ -628,9 +650,12 @@ __global__ void __launch_bounds__(WM* WN * 64, 2) ffn_ring_kernel(const FfnArgs<
   }
 }
 
-// The cut tiles: slabs added in order, then beta * C, rounded once.  Eight channels of one token per thread.
-template <typename TOut, int BM, int BN>
+// The cut tiles: slabs added in order, then scales, alpha and beta * C as in the ring's epilogue, rounded once.  Eight channels
+// of one token per thread.
+template <typename Tag, typename TOut, int BM, int BN>
 __global__ void __launch_bounds__(256) ffn_join_kernel(const FfnArgs<TOut> g) {
+  using Sum = typename FfnMma<Tag>::sum_t;
+  typedef Sum sum4 __attribute__((ext_vector_type(4)));
   const int64_t v = int64_t(blockIdx.x) * 256 + threadIdx.x;
   constexpr int PER_TILE = BM * BN / 8;
   const int t = int(v / PER_TILE), at = int(v % PER_TILE) * 8;  // (the grid is whole tiles)
@@ -638,33 +663,38 @@ __global__ void __launch_bounds__(256) ffn_join_kernel(const FfnArgs<TOut> g) {
   tile_coords(g.whole + t, g.tiles_m, g.tiles_n, tm, tn);
   const int64_t ch = int64_t(tm) * BM + at % BM, tok = int64_t(tn) * BN + at / BM;
   if (ch >= g.m || tok >= g.n) return;
-  const float* src = g.cube + int64_t(t) * g.slabs * (BM * BN) + at;
-  f32x4_t lo = *reinterpret_cast<const f32x4_t*>(src), hi = *reinterpret_cast<const f32x4_t*>(src + 4);
+  const Sum* src = static_cast<const Sum*>(g.cube) + int64_t(t) * g.slabs * (BM * BN) + at;
+  sum4 lo = *reinterpret_cast<const sum4*>(src), hi = *reinterpret_cast<const sum4*>(src + 4);
   for (int s = 1; s < g.slabs; ++s) {
     src += BM * BN;
-    lo += *reinterpret_cast<const f32x4_t*>(src);
-    hi += *reinterpret_cast<const f32x4_t*>(src + 4);
+    lo += *reinterpret_cast<const sum4*>(src);
+    hi += *reinterpret_cast<const sum4*>(src + 4);
   }
   TOut* out = g.c + ch + tok * g.ldc;
   const bool vec = ch + 8 <= g.m && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  constexpr int QUADS = int(sizeof(TOut)) / 2;  // 16-byte pieces of the eight results
   union {
     TOut e[8];
-    i32x4 q;
+    i32x4 q[QUADS];
   } x;
-  static_assert(sizeof(TOut) == 2, "16-bit results");
-  if (vec && !g.beta_zero) x.q = *reinterpret_cast<const i32x4*>(out);
+  if (vec && !g.beta_zero) {
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i) x.q[i] = reinterpret_cast<const i32x4*>(out)[i];
+  }
+  const float sb = g.scale_b ? g.scale_b[tok] : 1.0f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    float f = e < 4 ? lo[e & 3] : hi[e & 3];
-    if (vec) {
-      if (!g.beta_zero) f = f + g.beta * load_out(&x.e[e]);
-      store_out(&x.e[e], f);
-    } else if (ch + e < g.m) {
-      if (!g.beta_zero) f = f + g.beta * load_out(out + e);
-      store_out(out + e, f);
-    }
+    if (ch + e >= g.m) break;
+    const float sa = g.scale_a ? g.scale_a[ch + e] : 1.0f;
+    float f = g.alpha * ffn_scaled(e < 4 ? lo[e & 3] : hi[e & 3], sa, sb);
+    if (!g.beta_zero) f = f + g.beta * load_out(vec ? &x.e[e] : out + e);
+    if (vec) store_out(&x.e[e], f);
+    else store_out(out + e, f);
   }
-  if (vec) *reinterpret_cast<i32x4*>(out) = x.q;
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i) reinterpret_cast<i32x4*>(out)[i] = x.q[i];
+  }
 }
 
 // -------------------------------------------------------------------- repack
@@ -830,11 +860,12 @@ __global__ void __launch_bounds__(TPC < 256 ? 256 : TPC)
 
 // -------------------------------------------------- gradient, elementwise half
 // dG = dC U act'(G), dU = dC act(G): eight channels of one token per thread.  p and dp may be the same matrix: a thread
-// reads what it overwrites, and nothing else, before it writes.  (Hence no __restrict__ on them.)
+// reads what it overwrites, and nothing else, before it writes.  (Hence no __restrict__ on them.)  copy: NULL, or a second
+// dP with aligned rows of ld_copy (a multiple of 8) elements, zeros behind 2m, for products that need whole 16-byte pieces.
 template <typename Tag, typename TOut>
 __global__ void __launch_bounds__(256)
     ffn_gate_grad_kernel(int act, int64_t m, int64_t n, const uint16_t* p, int64_t ldp, const uint16_t* dc, int64_t lddc, uint16_t* dp,
-                         int64_t lddp) {
+                         int64_t lddp, uint16_t* copy, int64_t ld_copy) {
   const int64_t per = (m + 7) / 8;
   const int64_t v = int64_t(blockIdx.x) * 256 + threadIdx.x;
   if (v >= per * n) return;
@@ -842,6 +873,7 @@ __global__ void __launch_bounds__(256)
   const uint16_t* pg = p + col * ldp + i;
   const uint16_t* pd = dc + col * lddc + i;
   uint16_t* out = dp + col * lddp + i;
+  uint16_t* also = copy + col * ld_copy + i;
   with_act(act, [&](auto act_tag) {
   auto one = [&](uint16_t gb, uint16_t ub, uint16_t db, uint16_t& dg, uint16_t& du) {
     float value, slope;
@@ -866,15 +898,25 @@ __global__ void __launch_bounds__(256)
     }
     *reinterpret_cast<u16x8_at1*>(out) = og;
     *reinterpret_cast<u16x8_at1*>(out + m) = ou;
+    if (copy) {
+      *reinterpret_cast<u16x8_at1*>(also) = og;
+      *reinterpret_cast<u16x8_at1*>(also + m) = ou;
+    }
   } else {
     for (int e = 0; i + e < m; ++e) {
       uint16_t x, y;
       one(pg[e], pg[m + e], pd[e], x, y);
       out[e] = x;
       out[m + e] = y;
+      if (copy) {
+        also[e] = x;
+        also[m + e] = y;
+      }
     }
   }
   });
+  if (copy && i + 8 >= m)  // the thread of a token's last channels
+    for (int64_t e = 2 * m; e < ld_copy; ++e) copy[col * ld_copy + e] = 0;
 }
 
 }  // namespace sbamd

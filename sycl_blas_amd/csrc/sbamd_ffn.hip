@@ -63,9 +63,9 @@ hipError_t pack(Handle* h, const Rows& o, unsigned char* dst, int64_t row_bytes)
   return hipGetLastError();
 }
 
-template <typename Tag, typename TOut, bool GATED, bool CUT, bool TA, bool TB, int BM, int BN, int WM, int WN>
+template <typename Tag, typename TOut, bool GATED, bool TA, bool TB, int BM, int BN, int WM, int WN>
 hipError_t launch_ring(FfnArgs<TOut> g, int cus, hipStream_t stream) {
-  auto kernel = ffn_ring_kernel<Tag, TOut, GATED, CUT, TA, TB, BM, BN, WM, WN>;
+  auto kernel = ffn_ring_kernel<Tag, TOut, GATED, TA, TB, BM, BN, WM, WN>;
   constexpr int lds = ring_lds_bytes(BM, BN);
   static PerDeviceOnce lds_limit;
   const hipError_t e = lds_limit.run([&] {
@@ -77,48 +77,96 @@ hipError_t launch_ring(FfnArgs<TOut> g, int cus, hipStream_t stream) {
   if (tm > 0x7fff0000LL / tn) return hipErrorInvalidValue;
   g.tiles_m = int32_t(tm);
   g.tiles_n = int32_t(tn);
-  const int64_t resident = int64_t(cus) * (160 * 1024 / lds), units = CUT ? g.whole + (tm * tn - g.whole) * g.slabs : tm * tn;
+  const int64_t resident = int64_t(cus) * (160 * 1024 / lds), units = GATED ? tm * tn : g.whole + (tm * tn - g.whole) * g.slabs;
   if (units > 0x7fff0000LL) return hipErrorInvalidValue;
   hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(units, resident)), dim3(WM * WN * 64), lds, stream, g);
   return hipGetLastError();
 }
 
-template <typename Tag, typename TOut, bool GATED, bool CUT, int BM, int BN, int WM, int WN>
+template <typename Tag, typename TOut, bool GATED, int BM, int BN, int WM, int WN>
 hipError_t launch_ring_trans(const FfnArgs<TOut>& g, bool ta, bool tb, int cus, hipStream_t stream) {
   // 8-bit operands always lie along k here: the transposing LDS reads the other layouts need move 16-bit elements
   if constexpr (std::is_same<Tag, I8Tag>::value) {
-    return launch_ring<Tag, TOut, GATED, CUT, true, false, BM, BN, WM, WN>(g, cus, stream);
+    return launch_ring<Tag, TOut, GATED, true, false, BM, BN, WM, WN>(g, cus, stream);
   } else {
-    if (ta) return tb ? launch_ring<Tag, TOut, GATED, CUT, true, true, BM, BN, WM, WN>(g, cus, stream) : launch_ring<Tag, TOut, GATED, CUT, true, false, BM, BN, WM, WN>(g, cus, stream);
-    return tb ? launch_ring<Tag, TOut, GATED, CUT, false, true, BM, BN, WM, WN>(g, cus, stream) : launch_ring<Tag, TOut, GATED, CUT, false, false, BM, BN, WM, WN>(g, cus, stream);
+    if (ta) return tb ? launch_ring<Tag, TOut, GATED, true, true, BM, BN, WM, WN>(g, cus, stream) : launch_ring<Tag, TOut, GATED, true, false, BM, BN, WM, WN>(g, cus, stream);
+    return tb ? launch_ring<Tag, TOut, GATED, false, true, BM, BN, WM, WN>(g, cus, stream) : launch_ring<Tag, TOut, GATED, false, false, BM, BN, WM, WN>(g, cus, stream);
   }
 }
 
 inline bool aligned16(const void* p, int64_t ld_bytes) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld_bytes % 16 == 0; }
 
-// Which kernel: SBAMD_KERNEL_SMALL (narrow), _LARGE (128 x 128 ring) or _HUGE (256 x 256 ring), from estimated microseconds.
-// Lengths along k in bytes make one model of 8-bit and 16-bit operands: a fragment, a stage and a cache line hold the
-// same bytes, and a matrix instruction takes the same time for either.  Measured on MI355X over n = 16 ... 21504,
-// (k, m) = (1024, 4096), (4096, 1024), (4096, 4096), (4096, 16384), (16384, 4096), plain and gated:
-//   narrow: operands at 6.2 TB/s; what the workgroups (32 rows x up to 64 tokens) read again through L2 at 28 TB/s, 12
-//     where the tokens outgrow an XCD's 4 MB of it; 1.2e-3 per byte of k for a workgroup alone (rows 32768, 8192 bytes:
-//     n = 16 45 us, 48 58, 128 102; rows 8192: n = 224 43, 512 91);
-//   128 x 128: 3.3e-3 per byte of k with few tiles, 5.9e-3 with one per unit (8192 bytes: 33 / 51; 2048: 10 / 13.6), 5.5e-3
-//     per tile and unit beyond; operands at 4.4 TB/s;
+// How the ring works through the tiles of EDGE x EDGE: the first `whole` in one go, the rest in `slabs` pieces along k.
+struct RingPlan {
+  double time;  // estimated microseconds
+  int32_t whole, slabs;
+  int64_t chunk;
+};
+// Lengths along k in bytes make one model of 8-bit and 16-bit operands: a fragment, a stage and a cache line hold the same
+// bytes, and a matrix instruction takes the same time for either.  Measured on MI355X over n = 16 ... 21504, (k, m) = (1024, 4096),
+// (4096, 1024), (4096, 4096), (4096, 16384), (16384, 4096), plain and gated:
+//   128 x 128: 3.3e-3 us per byte of k with few tiles, 5.9e-3 with one per unit (8192 bytes: 33 / 51; 2048: 10 / 13.6), 6e-3 per
+//     tile and unit beyond (two share a unit, so no whole rounds: 448 tiles, 16384 bytes: 160); operands at 4.4 TB/s;
 //   256 x 256: 6 us and 13e-3 per byte and round of one tile per unit (2048 bytes, 10.5 rounds: 354; 8192: 1196), 8.2e-3
 //     with few units busy.
-inline int pick_ffn(int64_t rows, int64_t n, int64_t kb, int cus, double t_ring_extra) {
-  const double len = double(kb), bytes = double(rows + n) * len;
+// A tile count that leaves units idle in the last round (128 or 336 tiles of 256 x 256 on 256 units) has that round's tiles cut
+// along k into as many pieces as fill it, at the price of the pieces' sums going out and coming back (4.5 TB/s) and a second
+// launch.  (rows, n): the product's; len: bytes along k; cut: whether tiles may be cut.
+template <int EDGE>
+RingPlan plan_ring(int64_t rows, int64_t n, int64_t len, int cus, bool cut) {
+  const int64_t tiles = ceil_div(rows, EDGE) * ceil_div(n, EDGE), k = len / 2;
+  const double bytes = double(len), q = double(tiles) / cus;
+  auto one_round = [&](double share, double b) {  // with `share` of the units busy
+    return EDGE == 256 ? 6.0 + b * (8.2e-3 + 4.5e-3 * share) : b * (3.3e-3 + 2.6e-3 * share);
+  };
+  RingPlan best = {0.0, int32_t(std::min<int64_t>(tiles, 0x7fff0000LL)), 1, k};
+  const int64_t rounds = EDGE == 256 ? tiles / cus : 0, rest = tiles - rounds * cus;
+  const double t_whole = 3.0 + double(rounds) * (6.0 + bytes * 13e-3);
+  best.time = EDGE == 128 && q > 1.0 ? 3.0 + q * (bytes * 6.0e-3 + 0.7) : t_whole + (rest ? one_round(double(rest) / cus, bytes) : 0.0);
+  best.time = std::max(best.time, 3.0 + double(rows + n) * bytes / 4.4e6);
+  constexpr int64_t SHORTEST = 8 * RING_BK;  // a slab, in 16-bit units: below that its prologue costs more than its work
+  if (!cut || rest == 0 || k < 2 * SHORTEST || tiles > 0x7fff0000LL) return best;
+  for (int64_t s = 2; s <= 32 && s * rest <= cus; ++s) {
+    const int64_t chunk = RING_BK * ceil_div(k, RING_BK * s), slabs = ceil_div(k, chunk);
+    if (slabs < 2 || chunk < SHORTEST) continue;
+    const double cube = double(rest) * double(slabs) * EDGE * EDGE * 4.0;
+    const double t = t_whole + one_round(double(rest * slabs) / cus, 2.0 * double(chunk)) + 4.0 + 2.0 * cube / 4.5e6;
+    if (t < best.time) best = {t, int32_t(rounds * cus), int32_t(slabs), chunk};
+  }
+  return best;
+}
+
+// The narrow kernel: operands at 6.2 TB/s; what the workgroups (32 rows x up to 64 tokens) read again through L2 at 28 TB/s, 12
+// where the tokens outgrow an XCD's 4 MB of it; 1.2e-3 us per byte of k for a workgroup alone (rows 32768, 8192 bytes: n = 16
+// 45 us, 48 58, 128 102; rows 8192: n = 224 43, 512 91).
+inline double narrow_time(int64_t rows, int64_t n, int64_t len) {
+  const double b = double(len);
   const int64_t tok = n <= 16 ? 16 : n <= 32 ? 32 : n <= 48 ? 48 : 64;
   const double blocks = double(ceil_div(n, tok));
-  const double again = (double(ceil_div(rows, NARROW_ROWS)) * blocks * double(tok) + (blocks - 1.0) * double(rows)) * len;
-  const double t_narrow = 4.0 + std::max(len * 1.2e-3, bytes / 6.2e6 + again / (double(n) * len <= 4.5e6 ? 28e6 : 12e6));
-  const double q128 = double(ceil_div(rows, 128)) * double(ceil_div(n, 128)) / cus;
-  const double t_128 = t_ring_extra + 3.0 + std::max(q128 <= 1.0 ? len * (3.3e-3 + 2.6e-3 * q128) : std::ceil(q128) * (len * 5.5e-3 + 0.7), bytes / 4.4e6);
-  const double q256 = double(ceil_div(rows, 256)) * double(ceil_div(n, 256)) / cus, whole = std::floor(q256), part = q256 - whole;
-  const double t_256 = t_ring_extra + 3.0 + whole * (6.0 + len * 13e-3) + (part > 0.0 ? 6.0 + len * (8.2e-3 + 4.5e-3 * part) : 0.0);
-  if (t_narrow <= t_128 && t_narrow <= t_256) return SBAMD_KERNEL_SMALL;
-  return t_128 <= t_256 ? SBAMD_KERNEL_LARGE : SBAMD_KERNEL_HUGE;
+  const double again = (double(ceil_div(rows, NARROW_ROWS)) * blocks * double(tok) + (blocks - 1.0) * double(rows)) * b;
+  return 4.0 + std::max(b * 1.2e-3, double(rows + n) * b / 6.2e6 + again / (double(n) * b <= 4.5e6 ? 28e6 : 12e6));
+}
+
+// One ring launch by its plan, and the join of what it cut.  g has operands, sizes and outputs set.
+template <typename Tag, typename TOut, bool GATED, int EDGE, int WM, int WN>
+hipError_t run_ring(Handle* h, FfnArgs<TOut> g, bool ta, bool tb, int64_t rows, const RingPlan& plan, int cus) {
+  g.whole = plan.whole, g.slabs = plan.slabs, g.chunk = plan.chunk;
+  const int64_t tm = ceil_div(rows, EDGE), tn = ceil_div(g.n, EDGE), cut = GATED ? 0 : tm * tn - plan.whole;
+  hipError_t e = hipSuccess;
+  if (cut > 0) {
+    if ((e = ensure_scratch(h, size_t(cut) * size_t(plan.slabs) * EDGE * EDGE * sizeof(float))) != hipSuccess) return e;
+    g.cube = h->scratch;
+    h->last_depth = plan.slabs;
+    h->last_k_chunk = plan.chunk * 2 / FfnMma<Tag>::BYTES;
+  }
+  e = launch_ring_trans<Tag, TOut, GATED, EDGE, EDGE, WM, WN>(g, ta, tb, cus, h->stream);
+  if constexpr (!GATED) {
+    if (e != hipSuccess || cut <= 0) return e;
+    g.tiles_m = int32_t(tm), g.tiles_n = int32_t(tn);
+    hipLaunchKernelGGL((ffn_join_kernel<Tag, TOut, EDGE, EDGE>), dim3((unsigned)(cut * (EDGE * EDGE / 8 / 256))), dim3(256), 0, h->stream, g);
+    e = hipGetLastError();
+  }
+  return e;
 }
 
 // The product behind all forward entry points.
@@ -138,14 +186,16 @@ hipError_t run_ffn(Handle* h, const Rows& a, const Rows& b, FfnArgs<TOut> g) {
   // both operands, so a short or odd one is padded on both sides: the conditions on kb are the same for both.)
   const bool ring_pack_a = !ring_reads(a, GATED ? a.rows / 2 : a.rows), ring_pack_b = !ring_reads(b, b.rows);
   auto pack_time = [&](bool packed, const Rows& o) { return packed ? 3.0 + 2.0 * double(o.rows) * double(row_bytes) / 3.0e6 : 0.0; };
+  const RingPlan big = plan_ring<256>(a.rows, b.rows, row_bytes, cus, !GATED), small = plan_ring<128>(a.rows, b.rows, row_bytes, cus, !GATED);
   int family = h->kernel_override;
   if (family != SBAMD_KERNEL_SMALL && family != SBAMD_KERNEL_LARGE && family != SBAMD_KERNEL_HUGE) {
     const double extra = pack_time(ring_pack_a, a) + pack_time(ring_pack_b, b) - pack_time(a.across, a) - pack_time(b.across, b);
-    family = pick_ffn(a.rows, b.rows, kb, cus, extra);
+    const double t_ring = std::min(big.time, small.time);
+    family = narrow_time(a.rows, b.rows, kb) <= t_ring + extra ? SBAMD_KERNEL_SMALL : small.time <= big.time ? SBAMD_KERNEL_LARGE : SBAMD_KERNEL_HUGE;
   }
   if (kb == 0) family = SBAMD_KERNEL_SMALL;  // nothing to pipeline: the narrow kernel writes the sums over nothing
   const bool ring = family != SBAMD_KERNEL_SMALL;
-  const bool pack_a = ring ? ring_pack_a : a.across, pack_b = ring ? ring_pack_b : b.across;
+  const bool pack_a = kb > 0 && (ring ? ring_pack_a : a.across), pack_b = kb > 0 && (ring ? ring_pack_b : b.across);
   if (pack_a || pack_b) {
     const size_t bytes_a = pack_a ? size_t(a.rows) * size_t(row_bytes) : 0, bytes_b = pack_b ? size_t(b.rows) * size_t(row_bytes) : 0;
     const hipError_t e = ensure_aux(h, bytes_a + bytes_b);  // (rows of whole steps: b stays aligned behind a)
@@ -165,8 +215,8 @@ hipError_t run_ffn(Handle* h, const Rows& a, const Rows& b, FfnArgs<TOut> g) {
   const bool ta = pack_a || !a.across, tb = !pack_b && b.across;
 
   h->last_kernel = family;
-  if (family == SBAMD_KERNEL_HUGE) return launch_ring_trans<Tag, TOut, GATED, false, 256, 256, 2, 4>(g, ta, tb, cus, h->stream);
-  if (family == SBAMD_KERNEL_LARGE) return launch_ring_trans<Tag, TOut, GATED, false, 128, 128, 2, 2>(g, ta, tb, cus, h->stream);
+  if (family == SBAMD_KERNEL_HUGE) return run_ring<Tag, TOut, GATED, 256, 2, 4>(h, g, ta, tb, a.rows, big, cus);
+  if (family == SBAMD_KERNEL_LARGE) return run_ring<Tag, TOut, GATED, 128, 2, 2>(h, g, ta, tb, a.rows, small, cus);
   if (g.n <= 16) return launch_narrow<Tag, TOut, GATED, 1, 4, 2>(g, h->stream);
   if (g.n <= 32) return launch_narrow<Tag, TOut, GATED, 2, 2, 3>(g, h->stream);
   if (g.n <= 48) return launch_narrow<Tag, TOut, GATED, 3, 2, 2>(g, h->stream);
@@ -234,7 +284,7 @@ int forward(sbamd_handle_t hh, int act, char transa, char transb, int64_t m, int
   if (GATED && p && ldp < 2 * m) return SBAMD_INVALID_VALUE;
   if (m == 0 || n == 0) return SBAMD_OK;
   if (!c || (k > 0 && (!a || !b))) return SBAMD_INVALID_VALUE;
-  FfnArgs<TOut> g;
+  FfnArgs<TOut> g{};
   g.m = m, g.n = n;
   g.scale_a = scale_a, g.scale_b = scale_b;
   g.c = c, g.ldc = ldc;
@@ -290,72 +340,31 @@ struct Product {
   int64_t lim_b;  // see FfnArgs
 };
 
-// How the ring works through `tiles` tiles of EDGE x EDGE: the first `whole` in one go, the rest in `slabs` pieces along k.
-struct RingPlan {
-  double time;
-  int32_t whole, slabs;
-  int64_t chunk;
-};
-// Estimated microseconds as in pick_ffn; a tile count that leaves the last round of units mostly idle (128 or 336 tiles of
-// 256 x 256 on 256 units) has that round's tiles cut along k into as many pieces as fill it, at the price of the pieces' float sums
-// going out and coming back (4.5 TB/s) and a second launch.
-template <int EDGE>
-RingPlan plan_ring(int64_t m, int64_t n, int64_t k, int cus) {
-  const int64_t tiles = ceil_div(m, EDGE) * ceil_div(n, EDGE);
-  const double len = 2.0 * double(k), per_tile = EDGE == 256 ? 6.0 : 0.7, per_byte = EDGE == 256 ? 13e-3 : 5.5e-3;
-  auto round_of = [&](double share, double bytes) {  // one round with `share` of the units busy
-    return EDGE == 256 ? 6.0 + bytes * (8.2e-3 + 4.5e-3 * share) : 0.7 + bytes * (3.3e-3 + 2.6e-3 * share);
-  };
-  const int64_t rounds = tiles / cus, rest = tiles - rounds * cus;
-  const double t_whole = 3.0 + double(rounds) * (per_tile + len * per_byte);
-  RingPlan best = {t_whole + (rest ? round_of(double(rest) / cus, len) : 0.0), int32_t(std::min<int64_t>(tiles, 0x7fff0000LL)), 1, k};
-  if (rest == 0 || tiles > 0x7fff0000LL) return best;
-  for (int64_t s = 2; s <= 32 && s * rest <= cus; ++s) {
-    const int64_t chunk = RING_BK * ceil_div(k, RING_BK * s), slabs = ceil_div(k, chunk);
-    if (slabs < 2 || chunk < 8 * RING_BK) continue;
-    const double cube = double(rest) * double(slabs) * EDGE * EDGE * 4.0;
-    const double t = t_whole + round_of(double(rest * slabs) / cus, 2.0 * double(chunk)) + 4.0 + 2.0 * cube / 4.5e6;
-    if (t < best.time) best = {t, int32_t(rounds * cus), int32_t(slabs), chunk};
-  }
-  return best;
-}
-
-template <typename Tag, typename TOut, int EDGE, int WM, int WN>
-hipError_t run_ring_product(Handle* h, const Product<TOut>& q, const RingPlan& plan, int cus) {
-  FfnArgs<TOut> g{};
-  g.a = reinterpret_cast<const unsigned char*>(q.a), g.lda = q.lda * 2;
-  g.b = reinterpret_cast<const unsigned char*>(q.b), g.ldb = q.ldb * 2;
-  g.m = q.m, g.n = q.n, g.kb = q.k * 2;
-  g.c = q.c, g.ldc = q.ldc;
-  g.alpha = 1.0f, g.beta = q.beta, g.beta_zero = q.beta == 0.0f ? 1 : 0;
-  g.whole = plan.whole, g.slabs = plan.slabs, g.chunk = plan.chunk;
-  g.lim_b = q.lim_b;
-  const int64_t tm = ceil_div(q.m, EDGE), tn = ceil_div(q.n, EDGE), cut = tm * tn - plan.whole;
-  hipError_t e = hipSuccess;
-  if (cut > 0) {
-    if ((e = ensure_scratch(h, size_t(cut) * size_t(plan.slabs) * EDGE * EDGE * sizeof(float))) != hipSuccess) return e;
-    g.cube = static_cast<float*>(h->scratch);
-  }
-  e = launch_ring_trans<Tag, TOut, false, true, EDGE, EDGE, WM, WN>(g, q.ta, q.tb, cus, h->stream);
-  if (e != hipSuccess || cut <= 0) return e;
-  g.tiles_m = int32_t(tm), g.tiles_n = int32_t(tn);
-  hipLaunchKernelGGL((ffn_join_kernel<TOut, EDGE, EDGE>), dim3((unsigned)(cut * (EDGE * EDGE / 8 / 256))), dim3(256), 0, h->stream, g);
-  return hipGetLastError();
-}
-
 hipError_t run_product16(Handle* h, const Problem<uint16_t, uint16_t>& p, float beta) { return run_gemm_h(h, p, 1.0f, beta); }
 hipError_t run_product16(Handle* h, const Problem<uint16_t, bf16_bits>& p, float beta) { return run_gemm_b(h, p, 1.0f, beta); }
+
+template <typename TOut>
+bool ring_reads_product(const Product<TOut>& q) {
+  const int64_t lim_b = q.lim_b > 0 ? q.lim_b : q.n;
+  return aligned16(q.a, q.lda * 2) && aligned16(q.b, q.ldb * 2) && q.k >= RING_BK && (q.ta || q.m % 8 == 0) && (!q.tb || lim_b % 8 == 0);
+}
 
 template <typename Tag, typename TOut>
 hipError_t run_product(Handle* h, const Product<TOut>& q) {
   const int cus = h->compute_units > 0 ? h->compute_units : 256;
-  const int64_t lim_b = q.lim_b > 0 ? q.lim_b : q.n;
-  const bool ring = aligned16(q.a, q.lda * 2) && aligned16(q.b, q.ldb * 2) && q.k >= RING_BK && (q.ta || q.m % 8 == 0) && (!q.tb || lim_b % 8 == 0);
-  if (ring && h->kernel_override != SBAMD_KERNEL_SMALL) {
-    const RingPlan big = plan_ring<256>(q.m, q.n, q.k, cus), small = plan_ring<128>(q.m, q.n, q.k, cus);
+  if (ring_reads_product(q) && h->kernel_override != SBAMD_KERNEL_SMALL) {
+    const RingPlan big = plan_ring<256>(q.m, q.n, 2 * q.k, cus, true), small = plan_ring<128>(q.m, q.n, 2 * q.k, cus, true);
     const bool take_big = h->kernel_override == SBAMD_KERNEL_HUGE || (h->kernel_override != SBAMD_KERNEL_LARGE && big.time < small.time);
     h->last_kernel = take_big ? SBAMD_KERNEL_HUGE : SBAMD_KERNEL_LARGE;
-    return take_big ? run_ring_product<Tag, TOut, 256, 2, 4>(h, q, big, cus) : run_ring_product<Tag, TOut, 128, 2, 2>(h, q, small, cus);
+    FfnArgs<TOut> g{};
+    g.a = reinterpret_cast<const unsigned char*>(q.a), g.lda = q.lda * 2;
+    g.b = reinterpret_cast<const unsigned char*>(q.b), g.ldb = q.ldb * 2;
+    g.m = q.m, g.n = q.n, g.kb = q.k * 2;
+    g.c = q.c, g.ldc = q.ldc;
+    g.alpha = 1.0f, g.beta = q.beta, g.beta_zero = q.beta == 0.0f ? 1 : 0;
+    g.lim_b = q.lim_b;
+    return take_big ? run_ring<Tag, TOut, false, 256, 2, 4>(h, g, q.ta, q.tb, q.m, big, cus)
+                    : run_ring<Tag, TOut, false, 128, 2, 2>(h, g, q.ta, q.tb, q.m, small, cus);
   }
   // operands the ring cannot read as they lie: the 16-bit GEMM back end
   Problem<uint16_t, TOut> p{};
@@ -388,24 +397,50 @@ int gradient(sbamd_handle_t hh, int act, char transa, char transb, int64_t m, in
   if (tokens && (!p || !dc || !dp)) return SBAMD_INVALID_VALUE;
   if (dp == p && lddp != ldp) return SBAMD_INVALID_VALUE;  // in place means element for element
   if (tokens && k > 0 && ((da && !b) || (db && !a))) return SBAMD_INVALID_VALUE;
+  TOut* out_a = reinterpret_cast<TOut*>(da);
+  TOut* out_b = reinterpret_cast<TOut*>(db);
+  // the two products on a given dP (`lim`: how many elements of its rows may be read)
+  auto product_a = [&](const uint16_t* x, int64_t ldx, int64_t lim) -> Product<TOut> {
+    if (ta) return {bool(tb), true, k, 2 * m, n, b, ldb, x, ldx, beta_a, out_a, ldda, lim};
+    return {false, !tb, 2 * m, k, n, x, ldx, b, ldb, beta_a, out_a, ldda, 0};
+  };
+  auto product_b = [&](const uint16_t* x, int64_t ldx) -> Product<TOut> {
+    if (tb) return {true, bool(ta), n, k, 2 * m, x, ldx, a, lda, beta_b, out_b, lddb, 0};
+    return {!ta, false, k, n, 2 * m, a, lda, x, ldx, beta_b, out_b, lddb, 0};
+  };
+  const bool want_a = da && m > 0 && k > 0, want_b = db && n > 0 && k > 0;
+  // A dP whose rows do not come in whole 16-byte pieces keeps the ring from reading it (2 * 2730 rows, 1119 tokens, k = 1000:
+  // 47 us for dA against 29): the elementwise pass then writes a second, padded one into the handle's scratch area.
+  uint16_t* copy = nullptr;
+  const int64_t ld_copy = ceil_div(2 * m, 8) * 8;
+  if (tokens && h->kernel_override != SBAMD_KERNEL_SMALL) {
+    uint16_t* aligned = reinterpret_cast<uint16_t*>(uintptr_t(256));  // stands for the copy's place in the questions below
+    if ((want_a && !ring_reads_product(product_a(dp, lddp, 0)) && ring_reads_product(product_a(aligned, ld_copy, ld_copy))) ||
+        (want_b && !ring_reads_product(product_b(dp, lddp)) && ring_reads_product(product_b(aligned, ld_copy)))) {
+      const hipError_t e = ensure_aux(h, size_t(ld_copy) * size_t(n) * sizeof(uint16_t));
+      if (e != hipSuccess) return ffn_fail(h, e, "gradient scratch");
+      copy = static_cast<uint16_t*>(h->aux);
+    }
+  }
   if (tokens) {
     const int64_t grid = ceil_div(ceil_div(m, 8) * n, 256);
     if (grid > 0x7fffffffLL) return SBAMD_INVALID_VALUE;
-    hipLaunchKernelGGL((ffn_gate_grad_kernel<Tag, TOut>), dim3((unsigned)grid), dim3(256), 0, h->stream, act, m, n, p, ldp, dc, lddc, dp, lddp);
+    hipLaunchKernelGGL((ffn_gate_grad_kernel<Tag, TOut>), dim3((unsigned)grid), dim3(256), 0, h->stream, act, m, n, p, ldp, dc, lddc, dp, lddp, copy,
+                       ld_copy);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return ffn_fail(h, e, "gradient launch");
   }
   // The products run with n (m) == 0 too: a sum over nothing is beta times what was there.
-  TOut* out_a = reinterpret_cast<TOut*>(da);
-  TOut* out_b = reinterpret_cast<TOut*>(db);
-  if (da && m > 0 && k > 0) {
-    const hipError_t e = ta ? run_product<Tag, TOut>(h, {bool(tb), true, k, 2 * m, n, b, ldb, dp, lddp, beta_a, out_a, ldda, 0})
-                            : run_product<Tag, TOut>(h, {false, !tb, 2 * m, k, n, dp, lddp, b, ldb, beta_a, out_a, ldda, 0});
+  if (want_a) {
+    Product<TOut> q = product_a(dp, lddp, 0);
+    if (copy && !ring_reads_product(q) && ring_reads_product(product_a(copy, ld_copy, ld_copy))) q = product_a(copy, ld_copy, ld_copy);
+    const hipError_t e = run_product<Tag, TOut>(h, q);
     if (e != hipSuccess) return ffn_fail(h, e, "gradient product");
   }
-  if (db && n > 0 && k > 0) {
-    const hipError_t e = tb ? run_product<Tag, TOut>(h, {true, bool(ta), n, k, 2 * m, dp, lddp, a, lda, beta_b, out_b, lddb, 0})
-                            : run_product<Tag, TOut>(h, {!ta, false, k, n, 2 * m, a, lda, dp, lddp, beta_b, out_b, lddb, 0});
+  if (want_b) {
+    Product<TOut> q = product_b(dp, lddp);
+    if (copy && !ring_reads_product(q) && ring_reads_product(product_b(copy, ld_copy))) q = product_b(copy, ld_copy);
+    const hipError_t e = run_product<Tag, TOut>(h, q);
     if (e != hipSuccess) return ffn_fail(h, e, "gradient product");
   }
   return SBAMD_OK;

@@ -186,6 +186,15 @@ def test_scaled_families(h, family, n, m, k):
         assert h.last_kernel() == FAMILIES[family][0]
 
 
+@pytest.mark.parametrize("family", ["ring128", "ring256"])
+@pytest.mark.parametrize("n,m,k", [(300, 500, 4096), (130, 129, 5000), (70, 1030, 3333)])
+def test_scaled_cut_along_k(h, family, n, m, k):
+    """Few tiles and a long k: the tiles are cut along k and joined; whatever the cut, the integer sum is the same."""
+    for out, pad, beta in (("float32", 0, 0.0), ("bfloat16", 0, 0.5), ("float16", 3, 0.0), ("float32", 16, -1.5)):
+        run_scaled(h, out, n, m, k, alpha=0.01, beta=beta, pad=pad, family=FAMILIES[family])
+        assert h.last_splitk()[0] > 1
+
+
 @pytest.mark.parametrize("ta,tb", [("t", "n"), ("n", "n"), ("t", "t"), ("n", "t")])
 @pytest.mark.parametrize("n,m,k,pad,shift", [(5, 40, 70, 0, 0), (40, 90, 200, 3, 1), (129, 260, 96, 16, 0), (150, 300, 257, 1, 7)])
 def test_scaled_layouts(h, ta, tb, n, m, k, pad, shift):
@@ -207,9 +216,10 @@ def test_scaled_k_zero_and_alpha_zero(h, n):
     one = Mat(h, "int8", 1, 1)
     for beta, k, alpha in ((0.0, 0, 1.0), (2.0, 0, 1.0), (0.5, 9, 0.0), (0.0, 9, 0.0), (1.0, 9, 0.0)):
         start = values if beta else np.full_like(values, np.nan)
-        cg = Mat(h, "float32", n, m, m + 3, 0, start)
-        h.wait(sb._gemm_scaled(h, "t", "n", m, n, k, alpha, one.buf, k, None, one.buf, k, None, beta, cg.buf, cg.ld))
-        assert (cg.get() == np.float32(beta) * values).all(), (beta, k, alpha)
+        for ta, lda, tb, ldb in (("t", k, "n", k), ("n", m, "t", n)):
+            cg = Mat(h, "float32", n, m, m + 3, 0, start)
+            h.wait(sb._gemm_scaled(h, ta, tb, m, n, k, alpha, one.buf, lda, None, one.buf, ldb, None, beta, cg.buf, cg.ld))
+            assert (cg.get() == np.float32(beta) * values).all(), (beta, k, alpha, ta, tb)
 
 
 def test_scaled_largest_sums_are_exact(h):
