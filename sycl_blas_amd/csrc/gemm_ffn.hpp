@@ -544,12 +544,13 @@ __global__ void __launch_bounds__(WM* WN * 64, 2) ffn_ring_kernel(const FfnArgs<
     asm volatile("" : "+v"(lane_e));
     SBAMD_LDS unsigned char* corner = smem + (RING_STAGES - 1) * STAGE_BYTES + wave * CORNER_BYTES;
     const int tok = lane_e & 31, half = lane_e >> 5;
-    auto settle = [] {  // between the lanes' writes and other lanes' reads (one wavefront: LDS keeps its order)
+    auto settle = []() __attribute__((always_inline)) {  // between the lanes' writes and other lanes' reads (one wavefront: LDS keeps its order)
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
     };
+    // (always_inline below: a lambda that is called twice and left as a function would put the accumulators into memory)
     // the four floats of rows 8 Q + 4 half .. + 3 of the wavefront tile's 32-row block I, tokens of block J
-    auto four = [&](auto i_tag, auto j_tag, auto q_tag) {
+    auto four = [&](auto i_tag, auto j_tag, auto q_tag) __attribute__((always_inline)) {
       constexpr int I = decltype(i_tag)::value, J = decltype(j_tag)::value, Q = decltype(q_tag)::value;
       f32x4_t v;
 #pragma unroll
@@ -561,14 +562,14 @@ __global__ void __launch_bounds__(WM* WN * 64, 2) ffn_ring_kernel(const FfnArgs<
     };
     // value(i, q) of 32-channel blocks i = B0 .. B0 + BLOCKS - 1 of the wavefront's channels, through the corner to `out`
     auto emit_at = [&](auto sb_tag, auto j_tag, auto&& value, auto* out, int64_t ld, int64_t ch_at, int64_t ch_lim, int64_t tok_at,
-                       int64_t tok_lim, bool vec, bool read_c) {
+                       int64_t tok_lim, bool vec, bool read_c) __attribute__((always_inline)) {
       constexpr int SB = decltype(sb_tag)::value, J = decltype(j_tag)::value;
       using TTo = std::remove_pointer_t<decltype(out)>;
       constexpr int SLAB = CHW * SB < CORNER_ROW ? CHW : CORNER_ROW / SB, BLOCKS = SLAB / 32;
-      static_for<CHW / SLAB>([&](auto slab) {
+      static_for<CHW / SLAB>([&](auto slab) __attribute__((always_inline)) {
         constexpr int B0 = decltype(slab)::value * BLOCKS;
-        static_for<BLOCKS>([&](auto block) {
-          static_for<4>([&](auto q) {
+        static_for<BLOCKS>([&](auto block) __attribute__((always_inline)) {
+          static_for<4>([&](auto q) __attribute__((always_inline)) {
             const f32x4_t v = value(std::integral_constant<int, B0 + decltype(block)::value>{}, j_tag, q);
             const int at = corner_at(tok, (decltype(block)::value * 32 + decltype(q)::value * 8 + half * 4) * SB);
             if constexpr (SB == 4) {
@@ -590,7 +591,7 @@ __global__ void __launch_bounds__(WM* WN * 64, 2) ffn_ring_kernel(const FfnArgs<
         settle();
       });
     };
-    auto emit = [&](auto sb_tag, auto j_tag, auto&& value, TOut* out, int64_t ld, bool vec, bool read_c) {
+    auto emit = [&](auto sb_tag, auto j_tag, auto&& value, TOut* out, int64_t ld, bool vec, bool read_c) __attribute__((always_inline)) {
       emit_at(sb_tag, j_tag, value, out, ld, ch0, g.m, tok0, g.n, vec, read_c);
     };
     auto rows_aligned = [](const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (ld * int64_t(sizeof(TOut))) % 16 == 0; };
@@ -598,18 +599,18 @@ __global__ void __launch_bounds__(WM* WN * 64, 2) ffn_ring_kernel(const FfnArgs<
     using as_float = std::integral_constant<int, 4>;
     const bool vec_c = rows_aligned(g.c, g.ldc);
     if constexpr (GATED) {
-      auto gate = [&](auto i, auto j, auto q) { return four(std::integral_constant<int, 2 * decltype(i)::value>{}, j, q); };
-      auto up = [&](auto i, auto j, auto q) { return four(std::integral_constant<int, 2 * decltype(i)::value + 1>{}, j, q); };
+      auto gate = [&](auto i, auto j, auto q) __attribute__((always_inline)) { return four(std::integral_constant<int, 2 * decltype(i)::value>{}, j, q); };
+      auto up = [&](auto i, auto j, auto q) __attribute__((always_inline)) { return four(std::integral_constant<int, 2 * decltype(i)::value + 1>{}, j, q); };
       if (g.p) {
         const bool vec_p = rows_aligned(g.p, g.ldp);
-        static_for<NI>([&](auto j) {
+        static_for<NI>([&](auto j) __attribute__((always_inline)) {
           emit(own_size{}, j, gate, g.p, g.ldp, vec_p, false);
           emit(own_size{}, j, up, g.p + g.m, g.ldp, vec_p && rows_aligned(g.p + g.m, g.ldp), false);
         });
       }
-      with_act(g.act, [&](auto act) {
-        static_for<NI>([&](auto j_tag) {
-          emit(own_size{}, j_tag, [&](auto i, auto j, auto q) {
+      with_act(g.act, [&](auto act) __attribute__((always_inline)) {
+        static_for<NI>([&](auto j_tag) __attribute__((always_inline)) {
+          emit(own_size{}, j_tag, [&](auto i, auto j, auto q) __attribute__((always_inline)) {
             const f32x4_t x = gate(i, j, q), y = up(i, j, q);
             f32x4_t v;
 #pragma unroll
@@ -619,7 +620,7 @@ __global__ void __launch_bounds__(WM* WN * 64, 2) ffn_ring_kernel(const FfnArgs<
         });
       });
     } else {
-      auto scaled = [&](auto i, auto j, auto q) {
+      auto scaled = [&](auto i, auto j, auto q) __attribute__((always_inline)) {
         f32x4_t v = four(i, j, q);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = g.alpha * v[e];
@@ -627,7 +628,7 @@ __global__ void __launch_bounds__(WM* WN * 64, 2) ffn_ring_kernel(const FfnArgs<
       };
       if (partial) {
         float* tile_sums = static_cast<float*>(g.cube) + int64_t(piece_now) * (BM * BN);
-        auto sums = [&](auto i, auto j, auto q) {  // as they are (an integer's bits merely travel as a float's)
+        auto sums = [&](auto i, auto j, auto q) __attribute__((always_inline)) {  // as they are (an integer's bits merely travel as a float's)
           f32x4_t v;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -636,11 +637,11 @@ __global__ void __launch_bounds__(WM* WN * 64, 2) ffn_ring_kernel(const FfnArgs<
           }
           return v;
         };
-        static_for<NI>([&](auto j) { emit_at(as_float{}, j, sums, tile_sums, BM, wm * CHW, BM, wn * WTN, BN, true, false); });
+        static_for<NI>([&](auto j) __attribute__((always_inline)) { emit_at(as_float{}, j, sums, tile_sums, BM, wm * CHW, BM, wn * WTN, BN, true, false); });
       } else if (g.beta_zero) {
-        static_for<NI>([&](auto j) { emit(own_size{}, j, scaled, g.c, g.ldc, vec_c, false); });
+        static_for<NI>([&](auto j) __attribute__((always_inline)) { emit(own_size{}, j, scaled, g.c, g.ldc, vec_c, false); });
       } else {
-        static_for<NI>([&](auto j) { emit(as_float{}, j, scaled, g.c, g.ldc, vec_c, true); });
+        static_for<NI>([&](auto j) __attribute__((always_inline)) { emit(as_float{}, j, scaled, g.c, g.ldc, vec_c, true); });
       }
     }
     // (with P kept there are more stores than that: waiting for fewer is then merely early)
@@ -684,12 +685,16 @@ __global__ void __launch_bounds__(256) ffn_join_kernel(const FfnArgs<TOut> g) {
   const float sb = g.scale_b ? g.scale_b[tok] : 1.0f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    if (ch + e >= g.m) break;
-    const float sa = g.scale_a ? g.scale_a[ch + e] : 1.0f;
+    const bool live = ch + e < g.m;
+    const float sa = g.scale_a && live ? g.scale_a[ch + e] : 1.0f;
     float f = g.alpha * ffn_scaled(e < 4 ? lo[e & 3] : hi[e & 3], sa, sb);
-    if (!g.beta_zero) f = f + g.beta * load_out(vec ? &x.e[e] : out + e);
-    if (vec) store_out(&x.e[e], f);
-    else store_out(out + e, f);
+    if (vec) {
+      if (!g.beta_zero) f = f + g.beta * load_out(&x.e[e]);
+      store_out(&x.e[e], f);
+    } else if (live) {
+      if (!g.beta_zero) f = f + g.beta * load_out(out + e);
+      store_out(out + e, f);
+    }
   }
   if (vec) {
 #pragma unroll
@@ -698,40 +703,84 @@ __global__ void __launch_bounds__(256) ffn_join_kernel(const FfnArgs<TOut> g) {
 }
 
 // -------------------------------------------------------------------- repack
-// dst[r][0 .. row_bytes) = row r of the operand along k, zeros from `kb` bytes on.
-// ACROSS: element (r, k) of the source lies at r + k * ld (elements of BYTES bytes), transposed through a 64 x 64
-// LDS tile; else at k + r * ld (any alignment).  row_bytes is a multiple of 64.
-template <int BYTES, bool ACROSS>
+// dst[r][0 .. row_bytes) = row r of the operand along k, zeros from k on (elements of BYTES bytes; row_bytes a multiple of 64).
+// Bound by memory: the operand in and out once.
+//
+// Rows that lie along k already, at any alignment: one 16-byte piece per thread.
+template <int BYTES>
 __global__ void __launch_bounds__(256)
-    ffn_pack_kernel(const unsigned char* __restrict__ src, int64_t ld, unsigned char* __restrict__ dst, int64_t row_bytes, int64_t rows,
-                    int64_t k) {
-  using E = typename std::conditional<BYTES == 2, uint16_t, uint8_t>::type;
-  if constexpr (!ACROSS) {
-    const int64_t per = row_bytes / 16, v = int64_t(blockIdx.x) * 256 + threadIdx.x;
-    if (v >= per * rows) return;
-    const int64_t r = v / per, at = (v - r * per) * 16, kb = k * BYTES;
-    const unsigned char* s = src + r * ld * BYTES + at;
-    const int64_t left = kb - at;
-    const u16x8 out = partial_piece(s, int(left < 16 ? (left < 0 ? 0 : left) : 16), kb >= 16);
-    *reinterpret_cast<u16x8*>(dst + r * row_bytes + at) = out;
-  } else {
-    __shared__ E tile[64][64 + 4 / BYTES];
-    const int64_t kt = (row_bytes / BYTES + 63) / 64;
-    const int64_t r0 = int64_t(blockIdx.x) / kt * 64, k0 = int64_t(blockIdx.x) % kt * 64;
-    const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
-    const E* in = reinterpret_cast<const E*>(src);
+    ffn_pack_rows_kernel(const unsigned char* __restrict__ src, int64_t ld, unsigned char* __restrict__ dst, int64_t row_bytes, int64_t rows,
+                         int64_t k) {
+  const int64_t per = row_bytes / 16, v = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (v >= per * rows) return;
+  const int64_t r = v / per, at = (v - r * per) * 16, kb = k * BYTES;
+  const unsigned char* s = src + r * ld * BYTES + at;
+  const int64_t left = kb - at;
+  *reinterpret_cast<u16x8*>(dst + r * row_bytes + at) = partial_piece(s, int(left < 16 ? (left < 0 ? 0 : left) : 16), kb >= 16);
+}
+
+// Element (r, k) at r + k * ld: a tile of 256 bytes of rows by 128 bytes of k per workgroup.  A thread takes blocks of U x U elements
+// (U = 4 bytes' worth): U words of U rows each, one per k, turned in registers into U words of U k each, through LDS into
+// 16-byte pieces along k.  Whole cache lines both ways (8-bit 50400 x 4096: element by element 0.9 ms).
+constexpr int PACK_K_BYTES = 128, PACK_R_BYTES = 256;
+template <int BYTES>
+__global__ void __launch_bounds__(256)
+    ffn_pack_across_kernel(const unsigned char* __restrict__ src, int64_t ld, unsigned char* __restrict__ dst, int64_t row_bytes, int64_t rows,
+                           int64_t k) {
+  constexpr int U = 4 / BYTES, ROWS = PACK_R_BYTES / BYTES, KS = PACK_K_BYTES / BYTES;
+  constexpr int PITCH = PACK_K_BYTES + 4;  // bytes of a tile row in LDS
+  typedef uint32_t u32_at1 __attribute__((aligned(1)));
+  __shared__ uint32_t tile[ROWS * PITCH / 4];
+  const int64_t k_tiles = (row_bytes + PACK_K_BYTES - 1) / PACK_K_BYTES;
+  const int64_t r0 = int64_t(blockIdx.x) / k_tiles * ROWS, k0 = int64_t(blockIdx.x) % k_tiles * KS;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t r = r0 + lane * U;
+  uint32_t in[KS / U / 4][U];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int64_t kk = k0 + y + 4 * i, r = r0 + x;
-      tile[y + 4 * i][x] = kk < k && r < rows ? in[r + kk * ld] : E(0);
+  for (int b = 0; b < KS / U / 4; ++b)  // this wavefront's blocks along k: b * 4 + wave
+#pragma unroll
+    for (int e = 0; e < U; ++e) {
+      const int64_t kk = k0 + (b * 4 + wave) * U + e;
+      const unsigned char* s = src + (r + kk * ld) * BYTES;
+      uint32_t w = 0;
+      if (kk < k) {
+        if (r + U <= rows) {
+          w = *reinterpret_cast<const u32_at1*>(s);
+        } else {
+          for (int i = 0; r + i < rows; ++i)
+            for (int j = 0; j < BYTES; ++j) w |= uint32_t(s[i * BYTES + j]) << (8 * (i * BYTES + j));
+        }
+      }
+      in[b][e] = w;
     }
-    __syncthreads();
-    E* out = reinterpret_cast<E*>(dst);
-    const int64_t row_elems = row_bytes / BYTES;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int64_t r = r0 + y + 4 * i, kk = k0 + x;
-      if (r < rows && kk < row_elems) out[kk + r * row_elems] = tile[x][y + 4 * i];
+  for (int b = 0; b < KS / U / 4; ++b) {
+    uint32_t out[U];
+    if constexpr (BYTES == 2) {
+      out[0] = (in[b][0] & 0xffffu) | (in[b][1] << 16);
+      out[1] = (in[b][0] >> 16) | (in[b][1] & 0xffff0000u);
+    } else {
+      // bytes of (a, b): v_perm's selector counts the second operand's bytes 0-3, the first's 4-7
+      const uint32_t lo01 = __builtin_amdgcn_perm(in[b][1], in[b][0], 0x05010400u), lo23 = __builtin_amdgcn_perm(in[b][3], in[b][2], 0x05010400u);
+      const uint32_t hi01 = __builtin_amdgcn_perm(in[b][1], in[b][0], 0x07030602u), hi23 = __builtin_amdgcn_perm(in[b][3], in[b][2], 0x07030602u);
+      out[0] = (lo01 & 0xffffu) | (lo23 << 16);
+      out[1] = (lo01 >> 16) | (lo23 & 0xffff0000u);
+      out[2] = (hi01 & 0xffffu) | (hi23 << 16);
+      out[3] = (hi01 >> 16) | (hi23 & 0xffff0000u);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) tile[(lane * U + i) * (PITCH / 4) + b * 4 + wave] = out[i];
+  }
+  __syncthreads();
+  constexpr int PIECES = PACK_K_BYTES / 16;
+#pragma unroll
+  for (int i = 0; i < ROWS * PIECES / 256; ++i) {
+    const int p = i * 256 + threadIdx.x, row = p / PIECES, piece = p % PIECES;
+    const int64_t at = k0 * BYTES + piece * 16;
+    if (r0 + row < rows && at < row_bytes) {
+      const uint32_t* t = tile + row * (PITCH / 4) + piece * 4;
+      const i32x4 v = {int(t[0]), int(t[1]), int(t[2]), int(t[3])};
+      *reinterpret_cast<i32x4*>(dst + (r0 + row) * row_bytes + at) = v;
     }
   }
 }

@@ -54,12 +54,12 @@ struct Rows {
 template <int BYTES>
 hipError_t pack(Handle* h, const Rows& o, unsigned char* dst, int64_t row_bytes) {
   const unsigned char* src = static_cast<const unsigned char*>(o.x);
-  const int64_t grid = o.across ? ceil_div(o.rows, 64) * ceil_div(row_bytes / BYTES, 64) : ceil_div(row_bytes / 16 * o.rows, 256);
+  const int64_t grid = o.across ? ceil_div(o.rows, PACK_R_BYTES / BYTES) * ceil_div(row_bytes, PACK_K_BYTES) : ceil_div(row_bytes / 16 * o.rows, 256);
   if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
   if (o.across)
-    hipLaunchKernelGGL((ffn_pack_kernel<BYTES, true>), dim3((unsigned)grid), dim3(256), 0, h->stream, src, o.ld, dst, row_bytes, o.rows, o.k);
+    hipLaunchKernelGGL((ffn_pack_across_kernel<BYTES>), dim3((unsigned)grid), dim3(256), 0, h->stream, src, o.ld, dst, row_bytes, o.rows, o.k);
   else
-    hipLaunchKernelGGL((ffn_pack_kernel<BYTES, false>), dim3((unsigned)grid), dim3(256), 0, h->stream, src, o.ld, dst, row_bytes, o.rows, o.k);
+    hipLaunchKernelGGL((ffn_pack_rows_kernel<BYTES>), dim3((unsigned)grid), dim3(256), 0, h->stream, src, o.ld, dst, row_bytes, o.rows, o.k);
   return hipGetLastError();
 }
 
@@ -137,14 +137,16 @@ RingPlan plan_ring(int64_t rows, int64_t n, int64_t len, int cus, bool cut) {
 }
 
 // The narrow kernel: operands at 6.2 TB/s; what the workgroups (32 rows x up to 64 tokens) read again through L2 at 28 TB/s, 12
-// where the tokens outgrow an XCD's 4 MB of it; 1.2e-3 us per byte of k for a workgroup alone (rows 32768, 8192 bytes: n = 16
-// 45 us, 48 58, 128 102; rows 8192: n = 224 43, 512 91).
-inline double narrow_time(int64_t rows, int64_t n, int64_t len) {
+// where the tokens outgrow an XCD's 4 MB of it, both at 0.6 of that where rows are not 16-byte aligned; 3 us for each further
+// round of 512 workgroups (4550 of them with 64 bytes of k: 56); 1.2e-3 us per byte of k for a workgroup alone (rows 32768,
+// 8192 bytes: n = 16 45 us, 48 58, 128 102; rows 8192: n = 224 43, 512 91).
+inline double narrow_time(int64_t rows, int64_t n, int64_t len, bool aligned) {
   const double b = double(len);
   const int64_t tok = n <= 16 ? 16 : n <= 32 ? 32 : n <= 48 ? 48 : 64;
-  const double blocks = double(ceil_div(n, tok));
-  const double again = (double(ceil_div(rows, NARROW_ROWS)) * blocks * double(tok) + (blocks - 1.0) * double(rows)) * b;
-  return 4.0 + std::max(b * 1.2e-3, double(rows + n) * b / 6.2e6 + again / (double(n) * b <= 4.5e6 ? 28e6 : 12e6));
+  const double blocks = double(ceil_div(n, tok)), wgs = double(ceil_div(rows, NARROW_ROWS)) * blocks;
+  const double again = (wgs * double(tok) + (blocks - 1.0) * double(rows)) * b;
+  const double moved = double(rows + n) * b / 6.2e6 + again / (double(n) * b <= 4.5e6 ? 28e6 : 12e6);
+  return 4.0 + std::max(b * 1.2e-3, aligned ? moved : moved / 0.6) + 3.0 * std::max(0.0, wgs / 512.0 - 1.0);
 }
 
 // One ring launch by its plan, and the join of what it cut.  g has operands, sizes and outputs set.
@@ -191,7 +193,8 @@ hipError_t run_ffn(Handle* h, const Rows& a, const Rows& b, FfnArgs<TOut> g) {
   if (family != SBAMD_KERNEL_SMALL && family != SBAMD_KERNEL_LARGE && family != SBAMD_KERNEL_HUGE) {
     const double extra = pack_time(ring_pack_a, a) + pack_time(ring_pack_b, b) - pack_time(a.across, a) - pack_time(b.across, b);
     const double t_ring = std::min(big.time, small.time);
-    family = narrow_time(a.rows, b.rows, kb) <= t_ring + extra ? SBAMD_KERNEL_SMALL : small.time <= big.time ? SBAMD_KERNEL_LARGE : SBAMD_KERNEL_HUGE;
+    const bool rows_aligned = (a.across || aligned16(a.x, a.ld * BYTES)) && (b.across || aligned16(b.x, b.ld * BYTES));
+    family = narrow_time(a.rows, b.rows, kb, rows_aligned) <= t_ring + extra ? SBAMD_KERNEL_SMALL : small.time <= big.time ? SBAMD_KERNEL_LARGE : SBAMD_KERNEL_HUGE;
   }
   if (kb == 0) family = SBAMD_KERNEL_SMALL;  // nothing to pipeline: the narrow kernel writes the sums over nothing
   const bool ring = family != SBAMD_KERNEL_SMALL;
