@@ -12,6 +12,10 @@
 //   blas::helper::allocate / deallocate / copy_to_device / copy_to_host
 //                                   include/portblas_helper.h:54-67, :139-191
 //
+// Beside them, without a reference counterpart, the feed-forward layers of sbamd_ffn.h:
+//   blas::_quantize, _gemm_scaled, _gated_gemm, _gated_gemm_scaled,
+//   _gated_gemm_grad, activation_t
+//
 // Differences a caller sees: there is no sycl::queue -- SB_Handle is built from
 // a HIP device ordinal (and optionally a hipStream_t); buffers are created
 // through the handle; events wrap HIP events.  Argument errors throw the same
@@ -27,6 +31,7 @@
 #include <type_traits>
 #include <vector>
 
+#include "sbamd_ffn.h"
 #include "sbamd_gemm.h"
 
 namespace blas {
@@ -368,6 +373,135 @@ typename sb_handle_t::event_t _trsm(sb_handle_t& sb_handle, char side, char uplo
   sb_handle.depends_on(_dependencies);
   detail::check(api::trsm(sb_handle.native(), side, uplo, trans, diag, int64_t(M), int64_t(N), out_t(alpha),
                           detail::raw(A), int64_t(lda), detail::raw(B), int64_t(ldb)),
+                sb_handle.native());
+  return sb_handle.record();
+}
+
+// ------------------------------------------------- feed-forward layers (sbamd_ffn.h)
+enum class activation_t : int {
+  silu = SBAMD_ACT_SILU,
+  gelu = SBAMD_ACT_GELU,
+  gelu_tanh = SBAMD_ACT_GELU_TANH,
+  relu = SBAMD_ACT_RELU
+};
+
+namespace detail {
+// element type -> C-ABI entry points; `bits` is the C type its storage travels as
+template <typename T>
+struct ffn_abi;
+template <>
+struct ffn_abi<float> {
+  using bits = float;
+  static constexpr auto quantize = sbamd_squantize_i8;
+  static constexpr auto gemm_scaled = sbamd_i8sgemm;
+  static constexpr auto gated_scaled = sbamd_i8sgated_gemm;
+};
+template <>
+struct ffn_abi<half_t> {
+  using bits = uint16_t;
+  static constexpr auto quantize = sbamd_hquantize_i8;
+  static constexpr auto gemm_scaled = sbamd_i8hgemm;
+  static constexpr auto gated_scaled = sbamd_i8hgated_gemm;
+  static constexpr auto gated = sbamd_hgated_gemm;
+  static constexpr auto gated_grad = sbamd_hgated_gemm_grad;
+};
+template <>
+struct ffn_abi<bfloat16_t> {
+  using bits = uint16_t;
+  static constexpr auto quantize = sbamd_bquantize_i8;
+  static constexpr auto gemm_scaled = sbamd_i8bgemm;
+  static constexpr auto gated_scaled = sbamd_i8bgated_gemm;
+  static constexpr auto gated = sbamd_bgated_gemm;
+  static constexpr auto gated_grad = sbamd_bgated_gemm_grad;
+};
+template <typename T>
+typename ffn_abi<T>::bits* bits(T* p) {
+  return reinterpret_cast<typename ffn_abi<T>::bits*>(p);
+}
+template <typename T>
+const typename ffn_abi<T>::bits* bits(const T* p) {
+  return reinterpret_cast<const typename ffn_abi<T>::bits*>(p);
+}
+}  // namespace detail
+
+// Columns of the M x N matrix x to 8-bit integers with one float scale per column (sbamd_*quantize_i8).
+template <typename sb_handle_t, typename container_0_t, typename container_1_t, typename container_2_t, typename index_t>
+typename sb_handle_t::event_t _quantize(sb_handle_t& sb_handle, index_t _M, index_t _N, container_0_t x_, index_t _ldx, container_1_t q_,
+                                        index_t _ldq, container_2_t scale_,
+                                        const typename sb_handle_t::event_t& _dependencies = {}) {
+  using api = detail::ffn_abi<typename detail::elem<container_0_t>::type>;
+  sb_handle.depends_on(_dependencies);
+  detail::check(api::quantize(sb_handle.native(), int64_t(_M), int64_t(_N), detail::bits(detail::raw(x_)), int64_t(_ldx), detail::raw(q_),
+                              int64_t(_ldq), detail::raw(scale_)),
+                sb_handle.native());
+  return sb_handle.record();
+}
+
+// C <- alpha * diag(scale_a) * op(A) * op(B) * diag(scale_b) + beta * C, A and B int8_t; a scale may be a null
+// const float* (ones).
+template <typename sb_handle_t, typename container_0_t, typename container_1_t, typename container_2_t, typename container_3_t,
+          typename container_4_t, typename index_t>
+typename sb_handle_t::event_t _gemm_scaled(sb_handle_t& sb_handle, char _TransA, char _TransB, index_t _M, index_t _N, index_t _K,
+                                           float _alpha, container_0_t a_, index_t _lda, container_1_t scale_a, container_2_t b_,
+                                           index_t _ldb, container_3_t scale_b, float _beta, container_4_t _C, index_t _ldc,
+                                           const typename sb_handle_t::event_t& _dependencies = {}) {
+  using api = detail::ffn_abi<typename detail::elem<container_4_t>::type>;
+  sb_handle.depends_on(_dependencies);
+  detail::check(api::gemm_scaled(sb_handle.native(), _TransA, _TransB, int64_t(_M), int64_t(_N), int64_t(_K), _alpha, detail::raw(a_),
+                                 int64_t(_lda), detail::raw(scale_a), detail::raw(b_), int64_t(_ldb), detail::raw(scale_b), _beta,
+                                 detail::bits(detail::raw(_C)), int64_t(_ldc)),
+                sb_handle.native());
+  return sb_handle.record();
+}
+
+// C <- act(G) * U with (G; U) = op(A) * op(B), op(A) 2M x K; p_ (2M x N, or a null pointer of C's type) receives (G; U).
+template <typename sb_handle_t, typename container_0_t, typename container_1_t, typename container_2_t, typename container_3_t,
+          typename index_t>
+typename sb_handle_t::event_t _gated_gemm(sb_handle_t& sb_handle, activation_t act, char _TransA, char _TransB, index_t _M, index_t _N,
+                                          index_t _K, container_0_t a_, index_t _lda, container_1_t b_, index_t _ldb, container_2_t _C,
+                                          index_t _ldc, container_3_t p_, index_t _ldp,
+                                          const typename sb_handle_t::event_t& _dependencies = {}) {
+  using api = detail::ffn_abi<typename detail::elem<container_2_t>::type>;
+  sb_handle.depends_on(_dependencies);
+  detail::check(api::gated(sb_handle.native(), int(act), _TransA, _TransB, int64_t(_M), int64_t(_N), int64_t(_K),
+                           detail::bits(detail::raw(a_)), int64_t(_lda), detail::bits(detail::raw(b_)), int64_t(_ldb),
+                           detail::bits(detail::raw(_C)), int64_t(_ldc), detail::bits(detail::raw(p_)), int64_t(_ldp)),
+                sb_handle.native());
+  return sb_handle.record();
+}
+
+// The gated block on int8_t operands, scale_a with 2M entries.
+template <typename sb_handle_t, typename container_0_t, typename container_1_t, typename container_2_t, typename container_3_t,
+          typename container_4_t, typename index_t>
+typename sb_handle_t::event_t _gated_gemm_scaled(sb_handle_t& sb_handle, activation_t act, char _TransA, char _TransB, index_t _M,
+                                                 index_t _N, index_t _K, container_0_t a_, index_t _lda, container_1_t scale_a,
+                                                 container_2_t b_, index_t _ldb, container_3_t scale_b, container_4_t _C, index_t _ldc,
+                                                 const typename sb_handle_t::event_t& _dependencies = {}) {
+  using api = detail::ffn_abi<typename detail::elem<container_4_t>::type>;
+  sb_handle.depends_on(_dependencies);
+  detail::check(api::gated_scaled(sb_handle.native(), int(act), _TransA, _TransB, int64_t(_M), int64_t(_N), int64_t(_K), detail::raw(a_),
+                                  int64_t(_lda), detail::raw(scale_a), detail::raw(b_), int64_t(_ldb), detail::raw(scale_b),
+                                  detail::bits(detail::raw(_C)), int64_t(_ldc)),
+                sb_handle.native());
+  return sb_handle.record();
+}
+
+// Gradient of _gated_gemm; da_ or db_ may be a null pointer of the element type.
+template <typename sb_handle_t, typename container_0_t, typename container_1_t, typename container_2_t, typename container_3_t,
+          typename container_4_t, typename container_5_t, typename container_6_t, typename index_t>
+typename sb_handle_t::event_t _gated_gemm_grad(sb_handle_t& sb_handle, activation_t act, char _TransA, char _TransB, index_t _M, index_t _N,
+                                               index_t _K, container_0_t a_, index_t _lda, container_1_t b_, index_t _ldb,
+                                               container_2_t p_, index_t _ldp, container_3_t dc_, index_t _lddc, container_4_t dp_,
+                                               index_t _lddp, float _beta_a, container_5_t da_, index_t _ldda, float _beta_b,
+                                               container_6_t db_, index_t _lddb,
+                                               const typename sb_handle_t::event_t& _dependencies = {}) {
+  using api = detail::ffn_abi<typename detail::elem<container_4_t>::type>;
+  sb_handle.depends_on(_dependencies);
+  detail::check(api::gated_grad(sb_handle.native(), int(act), _TransA, _TransB, int64_t(_M), int64_t(_N), int64_t(_K),
+                                detail::bits(detail::raw(a_)), int64_t(_lda), detail::bits(detail::raw(b_)), int64_t(_ldb),
+                                detail::bits(detail::raw(p_)), int64_t(_ldp), detail::bits(detail::raw(dc_)), int64_t(_lddc),
+                                detail::bits(detail::raw(dp_)), int64_t(_lddp), _beta_a, detail::bits(detail::raw(da_)), int64_t(_ldda),
+                                _beta_b, detail::bits(detail::raw(db_)), int64_t(_lddb)),
                 sb_handle.native());
   return sb_handle.record();
 }

@@ -276,7 +276,8 @@ __global__ void __launch_bounds__(NARROW_WAVES * 64, OCC) ffn_narrow_kernel(cons
   // starts 6.1; rows of 16384: 5.7 / 4.9 / 6.1; 32768: 5.4 / 5.0 / 6.0).  The order of a row's sum is fixed by its place.
   const int64_t whole = g.kb / NARROW_CHUNK;
   const int64_t first = whole * wave / W, count = whole * (wave + 1) / W - first;
-  const int64_t turn = count > 0 ? (int64_t(tm) * 8 + wave * 2) % count : 0;
+  const uint32_t turns = uint32_t(count < 0x7fffffff ? count : 0x7fffffff);
+  const int64_t turn = count > 0 ? (uint32_t(tm) * 8u + uint32_t(wave) * 2u) % turns : 0;
   auto chunk = [&](int64_t i) {
     i += turn;
     return first + (i < count ? i : i - count);

@@ -44,15 +44,22 @@ static void release_retired(Handle* h, bool all) {
 // freed later, once that event has completed.  The handle's stream is not waited
 // for here (hipMalloc, and the hipFree of a parked buffer whose event has already
 // completed, are the only runtime calls that may block).
-static hipError_t grow(Handle* h, void** buf, size_t* have, size_t bytes) {
+static hipError_t grow(Handle* h, void** buf, size_t* have, bool* in_graph, size_t bytes) {
   std::lock_guard<std::mutex> lock(h->mu);
-  if (bytes <= *have) return hipSuccess;
-  release_retired(h, false);
+  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+  const bool capturing = hipStreamIsCapturing(h->stream, &capture) == hipSuccess && capture == hipStreamCaptureStatusActive;
+  if (bytes <= *have) {
+    *in_graph = *in_graph || capturing;
+    return hipSuccess;
+  }
+  if (!capturing) release_retired(h, false);
   const size_t rounded = (bytes + (size_t(1) << 20) - 1) & ~((size_t(1) << 20) - 1);
   void* fresh = nullptr;
   hipError_t e = hipMalloc(&fresh, rounded);
   if (e != hipSuccess) return e;
-  if (*buf) {
+  if (*buf && *in_graph) {
+    h->captured.push_back(*buf);
+  } else if (*buf) {
     hipEvent_t done;
     e = hipEventCreateWithFlags(&done, hipEventDisableTiming);
     if (e == hipSuccess) e = hipEventRecord(done, h->stream);
@@ -64,6 +71,7 @@ static hipError_t grow(Handle* h, void** buf, size_t* have, size_t bytes) {
   }
   *buf = fresh;
   *have = rounded;
+  *in_graph = capturing;
   return hipSuccess;
 }
 
@@ -85,8 +93,8 @@ static hipError_t fixed_scratch_of(int device, void** out) {
   return hipSuccess;
 }
 
-hipError_t ensure_scratch(Handle* h, size_t bytes) { return grow(h, &h->scratch, &h->scratch_bytes, bytes); }
-hipError_t ensure_aux(Handle* h, size_t bytes) { return grow(h, &h->aux, &h->aux_bytes, bytes); }
+hipError_t ensure_scratch(Handle* h, size_t bytes) { return grow(h, &h->scratch, &h->scratch_bytes, &h->scratch_captured, bytes); }
+hipError_t ensure_aux(Handle* h, size_t bytes) { return grow(h, &h->aux, &h->aux_bytes, &h->aux_captured, bytes); }
 
 namespace {
 
@@ -356,6 +364,7 @@ int sbamd_destroy(sbamd_handle_t h) {
   }
   if (h->impl.scratch) (void)hipFree(h->impl.scratch);
   if (h->impl.aux) (void)hipFree(h->impl.aux);
+  for (void* p : h->impl.captured) (void)hipFree(p);
   if (h->impl.owns_stream) (void)hipStreamDestroy(h->impl.stream);
   delete h;
   return SBAMD_OK;

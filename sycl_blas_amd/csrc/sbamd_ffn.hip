@@ -251,11 +251,11 @@ hipError_t scale_c<bf16_bits>(Handle* h, bf16_bits* c, int64_t m, int64_t n, int
   return hipGetLastError();
 }
 
-// Sizes and leading dimensions shared by the forward entry points; SBAMD_OK and `done` when there is nothing to write.
-int check_sizes(int ta, int tb, int64_t rows_a, int64_t m, int64_t n, int64_t k, int64_t lda, int64_t ldb, int64_t ldc) {
-  (void)m;
-  if (lda < (ta ? k : rows_a) || ldb < (tb ? n : k) || ldc < m) return SBAMD_INVALID_VALUE;
-  return SBAMD_OK;
+// Is `ld` a leading dimension for `rows` rows, and does a matrix of `cols` such columns of `bytes`-byte elements have a size that
+// address arithmetic can hold at all?
+bool holds(int64_t ld, int64_t rows, int64_t cols, int64_t bytes) {
+  int64_t size = 0;
+  return ld >= rows && !__builtin_mul_overflow(ld, cols, &size) && !__builtin_mul_overflow(size, bytes, &size) && size < (int64_t(1) << 60);
 }
 
 template <typename Tag, typename TOut, bool GATED>
@@ -264,7 +264,7 @@ int forward(sbamd_handle_t hh, int act, char transa, char transb, int64_t m, int
             TOut* p, int64_t ldp) {
   if (!hh) return SBAMD_INVALID_HANDLE;
   Handle* h = &hh->impl;
-  // (2m and byte counts along k have to fit 63 bits)
+  // (so that 2m and sums of sizes stay far from 63 bits; the matrices' own sizes are checked below)
   constexpr int64_t LIMIT = int64_t(1) << 40;
   if (m < 0 || n < 0 || k < 0 || m > LIMIT || n > LIMIT || k > LIMIT) return SBAMD_INVALID_VALUE;
   if (GATED && (act < SBAMD_ACT_SILU || act > SBAMD_ACT_RELU)) return SBAMD_INVALID_VALUE;
@@ -273,7 +273,7 @@ int forward(sbamd_handle_t hh, int act, char transa, char transb, int64_t m, int
   forget_last(h, k);
   if (!GATED && alpha == 0.0f) {  // as in GEMM: before the trans flags, A and B are not read
     if (m == 0 || n == 0) return SBAMD_OK;
-    if (!c || ldc < m) return SBAMD_INVALID_VALUE;
+    if (!c || !holds(ldc, m, n, sizeof(TOut))) return SBAMD_INVALID_VALUE;
     if (beta == 1.0f) return SBAMD_OK;
     const hipError_t e = scale_c<TOut>(h, c, m, n, ldc, beta);
     return e == hipSuccess ? SBAMD_OK : ffn_fail(h, e, "scale launch");
@@ -283,8 +283,10 @@ int forward(sbamd_handle_t hh, int act, char transa, char transb, int64_t m, int
   if (tb < 0) return SBAMD_INVALID_TRANSB;
   if (std::is_same<Tag, I8Tag>::value && k > SBAMD_I8_MAX_K) return SBAMD_NOT_SUPPORTED;
   const int64_t rows_a = GATED ? 2 * m : m;
-  if (check_sizes(ta, tb, rows_a, m, n, k, lda, ldb, ldc) != SBAMD_OK) return SBAMD_INVALID_VALUE;
-  if (GATED && p && ldp < 2 * m) return SBAMD_INVALID_VALUE;
+  constexpr int64_t BYTES = FfnMma<Tag>::BYTES, BYTES_C = sizeof(TOut);
+  if (!holds(lda, ta ? k : rows_a, ta ? rows_a : k, BYTES) || !holds(ldb, tb ? n : k, tb ? k : n, BYTES) || !holds(ldc, m, n, BYTES_C))
+    return SBAMD_INVALID_VALUE;
+  if (GATED && p && !holds(ldp, 2 * m, n, BYTES_C)) return SBAMD_INVALID_VALUE;
   if (m == 0 || n == 0) return SBAMD_OK;
   if (!c || (k > 0 && (!a || !b))) return SBAMD_INVALID_VALUE;
   FfnArgs<TOut> g{};
@@ -315,7 +317,7 @@ int quantize(sbamd_handle_t hh, int64_t m, int64_t n, const typename QuantIn<Tag
              float* scale) {
   if (!hh) return SBAMD_INVALID_HANDLE;
   Handle* h = &hh->impl;
-  if (m < 0 || n < 0 || ldx < m || ldq < m) return SBAMD_INVALID_VALUE;
+  if (m < 0 || n < 0 || !holds(ldx, m, n, sizeof(typename QuantIn<Tag>::type)) || !holds(ldq, m, n, 1)) return SBAMD_INVALID_VALUE;
   DeviceGuard guard(h->device);
   if (!guard.ok) return SBAMD_HIP_ERROR;
   forget_last(h, 0);
@@ -394,8 +396,10 @@ int gradient(sbamd_handle_t hh, int act, char transa, char transb, int64_t m, in
   if (ta < 0) return SBAMD_INVALID_TRANSA;
   if (tb < 0) return SBAMD_INVALID_TRANSB;
   const int64_t rows_a = ta ? k : 2 * m, rows_b = tb ? n : k;
-  if (ldp < 2 * m || lddc < m || lddp < 2 * m || (da && ldda < rows_a) || (db && lddb < rows_b)) return SBAMD_INVALID_VALUE;
-  if ((da && ldb < rows_b) || (db && lda < rows_a)) return SBAMD_INVALID_VALUE;
+  const int64_t cols_a = ta ? 2 * m : k, cols_b = tb ? k : n;
+  if (!holds(ldp, 2 * m, n, 2) || !holds(lddc, m, n, 2) || !holds(lddp, 2 * m, n, 2)) return SBAMD_INVALID_VALUE;
+  if (da && (!holds(ldda, rows_a, cols_a, 2) || !holds(ldb, rows_b, cols_b, 2))) return SBAMD_INVALID_VALUE;
+  if (db && (!holds(lddb, rows_b, cols_b, 2) || !holds(lda, rows_a, cols_a, 2))) return SBAMD_INVALID_VALUE;
   const bool tokens = m > 0 && n > 0;  // is there a dP at all?
   if (tokens && (!p || !dc || !dp)) return SBAMD_INVALID_VALUE;
   if (dp == p && lddp != ldp) return SBAMD_INVALID_VALUE;  // in place means element for element

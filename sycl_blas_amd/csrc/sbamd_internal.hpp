@@ -47,6 +47,10 @@ struct Handle {
     hipEvent_t done;
   };
   std::vector<Retired> retired;
+  // A graph replays with the buffers its calls were captured with: a buffer handed out while the stream captures is
+  // kept until the handle goes, also when a later call outgrows it.
+  bool scratch_captured = false, aux_captured = false;
+  std::vector<void*> captured;
   // This device's address of the fixed array that the entry point which allocates
   // nothing keeps its split-K cube in (looked up once, in sbamd_create).
   void* fixed_scratch = nullptr;

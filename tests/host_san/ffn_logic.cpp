@@ -38,6 +38,18 @@ int main() {
   auto* q = static_cast<int8_t*>(room);
   const int64_t far = int64_t(1) << 41;
 
+  // ---- leading dimensions whose matrices no address space holds
+  const int64_t huge = int64_t(1) << 62;
+  REFUSED(SBAMD_INVALID_VALUE, sbamd_squantize_i8(h, 4, 4, f, huge, q, 4, f));
+  REFUSED(SBAMD_INVALID_VALUE, sbamd_squantize_i8(h, 4, 4, f, 4, q, huge, f));
+  REFUSED(SBAMD_INVALID_VALUE, sbamd_i8sgemm(h, 't', 'n', 4, 4, 4, 1, q, huge, f, q, 4, f, 0, f, 4));
+  REFUSED(SBAMD_INVALID_VALUE, sbamd_i8sgemm(h, 't', 'n', 4, 4, 4, 1, q, 4, f, q, huge, f, 0, f, 4));
+  REFUSED(SBAMD_INVALID_VALUE, sbamd_i8sgemm(h, 't', 'n', 4, 4, 4, 1, q, 4, f, q, 4, f, 0, f, huge));
+  REFUSED(SBAMD_INVALID_VALUE, sbamd_i8sgemm(h, 't', 'n', 4, 4, 4, 0, q, 4, f, q, 4, f, 0, f, huge));
+  REFUSED(SBAMD_INVALID_VALUE, sbamd_bgated_gemm(h, SBAMD_ACT_SILU, 't', 'n', 4, 4, 4, u, 4, u, 4, u, 4, u, huge));
+  REFUSED(SBAMD_INVALID_VALUE, sbamd_bgated_gemm_grad(h, SBAMD_ACT_SILU, 't', 'n', 4, 4, 4, u, 4, u, 4, u, 8, u, huge, u, 8, 0, u, 4, 0, u, 4));
+  REFUSED(SBAMD_INVALID_VALUE, sbamd_bgated_gemm_grad(h, SBAMD_ACT_SILU, 't', 'n', 4, 4, 4, u, huge, u, 4, u, 8, u, 4, u, 8, 0, u, 4, 0, u, 4));
+
   // ---- quantisation
   REFUSED(SBAMD_INVALID_HANDLE, sbamd_squantize_i8(nullptr, 4, 4, f, 4, q, 4, f));
   REFUSED(SBAMD_INVALID_VALUE, sbamd_squantize_i8(h, -1, 4, f, 4, q, 4, f));

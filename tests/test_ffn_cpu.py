@@ -72,6 +72,48 @@ def test_element_types_are_checked_before_the_call():
             call()
 
 
+CALLS = r"""
+#include "portblas_compat.hpp"
+template <typename T>
+void layer(blas::SB_Handle& h) {
+  using blas::activation_t;
+  auto x = blas::make_sycl_iterator_buffer<T>(h, 64), y = blas::make_sycl_iterator_buffer<T>(h, 64);
+  auto q = blas::make_sycl_iterator_buffer<int8_t>(h, 64);
+  auto s = blas::make_sycl_iterator_buffer<float>(h, 64);
+  const float* ones = nullptr;
+  auto ev = blas::_quantize(h, 4, 4, x, 4, q, 4, s);
+  ev = blas::_gemm_scaled(h, 't', 'n', 4, 4, 4, 1.0f, q, 4, s, q, 4, ones, 0.0f, y, 4, ev);
+  blas::_gated_gemm_scaled(h, activation_t::gelu, 't', 'n', 2, 4, 4, q, 4, s, q, 4, s, y, 2, ev);
+}
+template <typename T>
+void training(blas::SB_Handle& h) {
+  using blas::activation_t;
+  auto w = blas::make_sycl_iterator_buffer<T>(h, 64), x = w, c = w, p = w, dw = w, dx = w;
+  T* none = nullptr;
+  auto ev = blas::_gated_gemm(h, activation_t::silu, 't', 'n', 2, 4, 4, w, 4, x, 4, c, 2, p + 8, 4);
+  blas::_gated_gemm(h, activation_t::silu, 't', 'n', 2, 4, 4, w, 4, x.get(), 4, c, 2, none, 0, ev);
+  blas::_gated_gemm_grad(h, activation_t::silu, 't', 'n', 2, 4, 4, w, 4, x, 4, p, 4, c, 2, p, 4, 0.0f, dw, 4, 1.0f, none, 4, ev);
+}
+int main() {
+  blas::SB_Handle h(0);
+  layer<float>(h);
+  layer<blas::half_t>(h);
+  layer<blas::bfloat16_t>(h);
+  training<blas::half_t>(h);
+  training<blas::bfloat16_t>(h);
+}
+"""
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs g++")
+def test_cpp_interface_compiles_for_every_type(tmp_path):
+    source = tmp_path / "calls.cpp"
+    source.write_text(CALLS)
+    run = subprocess.run(["g++", "-std=c++17", "-Wall", "-Werror", "-fsyntax-only", "-I", os.path.join(ROOT, "include"), str(source)],
+                         capture_output=True, text=True)
+    assert run.returncode == 0, run.stderr[-3000:]
+
+
 @pytest.mark.skipif(not os.path.exists("/opt/rocm/bin/hipcc") or shutil.which("make") is None, reason="needs hipcc and make")
 def test_host_logic_refuses_and_accepts_under_asan_and_ubsan():
     build = subprocess.run(["make", "-C", HOST_SAN, "-j8", "build/ffn_logic"], capture_output=True, text=True)

@@ -733,6 +733,59 @@ def test_captured_layer_replays(h):
         hh.close()
 
 
+def test_captured_call_keeps_its_scratch(h):
+    """A call that repacks an operand and one that cuts its product along k, captured into a graph; a later, bigger call
+    outgrows the scratch they were captured with; the graph still replays right."""
+    hip = C.CDLL("libamdhip64.so")
+    n, m, k = 200, 300, 2048
+    hh = sb.SB_Handle(0)
+    graph, graph_exec = C.c_void_p(), C.c_void_p()
+    rng = seeded("captured scratch")
+    x, w = int8_operands(rng, n, m, k)
+    xg, wg = Mat(hh, "int8", n, k, values=x), Mat(hh, "int8", k, m, values=across(w))
+    c = Mat(hh, "float32", n, m)
+    big_x, big_w = int8_operands(rng, 2 * n, 4 * m, 2 * k)
+    big = [Mat(hh, "int8", 2 * n, 2 * k, values=big_x), Mat(hh, "int8", 2 * k, 4 * m, values=across(big_w)), Mat(hh, "float32", 2 * n, 4 * m)]
+    want = (x.astype(np.int64) @ w.astype(np.int64).T).astype(np.float32)
+    hh.set_kernel(*RING128)
+
+    def call():
+        assert _lib.load().sbamd_i8sgemm(hh._h, b"n", b"n", m, n, k, 1.0, wg.buf.ptr, m, None, xg.buf.ptr, k, None, 0.0, c.buf.ptr,
+                                         m) == _lib.OK
+
+    try:
+        call()  # the scratch has to exist before the capture
+        assert hh.last_splitk()[0] > 1
+        hh.wait()
+        stream = C.c_void_p(hh.get_stream())
+        assert hip.hipStreamBeginCapture(stream, 0) == 0
+        call()
+        assert hip.hipStreamEndCapture(stream, C.byref(graph)) == 0 and graph.value
+        assert hip.hipGraphInstantiate(C.byref(graph_exec), graph, None, None, 0) == 0
+        for i in range(4):
+            hh.wait(sb._gemm_scaled(hh, "n", "n", 4 * m, 2 * n, 2 * k, 1.0, big[1].buf, 4 * m, None, big[0].buf, 2 * k, None, 0.0,
+                                    big[2].buf, 4 * m))
+            assert (big[2].get() == (big_x.astype(np.int64) @ big_w.astype(np.int64).T).astype(np.float32)).all()
+            filler = helper.allocate(hh, "float32", 1 << 20)  # lands where a freed scratch buffer would have been
+            helper.copy_to_device(hh, np.full(1 << 20, np.nan, np.float32), filler)
+            hh.wait(helper.copy_to_device(hh, np.zeros((n, m), np.float32), c.buf, n * m))
+            assert hip.hipGraphLaunch(graph_exec, stream) == 0
+            hh.wait()
+            got = np.empty_like(c.host)
+            hh.wait(helper.copy_to_host(hh, c.alloc, got))
+            assert (c.window(got) == want).all(), f"replay {i}"
+            helper.deallocate(filler)
+    finally:
+        if graph_exec.value:
+            hip.hipGraphExecDestroy(graph_exec)
+        if graph.value:
+            hip.hipGraphDestroy(graph)
+        hh.wait()
+        for mat in (xg, wg, c, *big):
+            helper.deallocate(mat.alloc)
+        hh.close()
+
+
 # -------------------------------------------------------------------- refusals
 def test_refusals_leave_the_output(h):
     i8, f = Mat(h, "int8", 4, 8), Mat(h, "float32", 4, 8)
