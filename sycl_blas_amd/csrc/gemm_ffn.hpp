@@ -96,11 +96,35 @@ __device__ inline float ffn_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f
 // tanh(y) = 2 sigmoid(2y) - 1, so 0.5 g (1 + tanh(y)) = g sigmoid(2y), without the cancellation for negative g.
 __device__ inline float gelu_tanh_arg2(float g) { return 1.5957691216057308f * (g + 0.044715f * g * g * g); }
 
+// Phi(g) and e^(-g^2/2), one exponential for both: with x = |g| / sqrt(2), erfc(x) = e^(-x^2) R(x), and R is a polynomial in
+// t = 1 / (1 + 0.4 x), fitted for the least largest relative error over 0 <= x <= 9.5 (8.4e-8; 4.3e-7 as evaluated in float), so the
+// small values of Phi far on the negative side keep their relative precision, which 1 + erf would cancel away.
+// (The device library's erfc took two thirds of the elementwise gradient's time for this activation.)
+__device__ inline void normal_parts(float g, float& phi, float& bell) {
+  const float x = __builtin_fabsf(g) * 0.70710678118654752f;
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.4f, x, 1.0f));
+  float r = 0.07275442034006119f;
+  r = __builtin_fmaf(r, t, -0.39065292477607727f);
+  r = __builtin_fmaf(r, t, 0.685164749622345f);
+  r = __builtin_fmaf(r, t, -0.38698726892471313f);
+  r = __builtin_fmaf(r, t, 0.4279186427593231f);
+  r = __builtin_fmaf(r, t, 0.12624987959861755f);
+  r = __builtin_fmaf(r, t, 0.24152310192584991f);
+  r = __builtin_fmaf(r, t, 0.22394883632659912f);
+  r = __builtin_fmaf(r, t, 8.045712456805632e-05f);
+  bell = __builtin_amdgcn_exp2f(-0.72134752044448170f * g * g);
+  const float tail = 0.5f * bell * r;
+  phi = g < 0.0f ? tail : 1.0f - tail;
+}
+
 template <int ACT>
 __device__ inline float act_value(float g) {
   if constexpr (ACT == SBAMD_ACT_SILU) return g * ffn_sigmoid(g);
-  else if constexpr (ACT == SBAMD_ACT_GELU) return 0.5f * g * erfcf(-0.70710678118654752f * g);  // 2 Phi(g) = erfc(-g / sqrt(2))
-  else if constexpr (ACT == SBAMD_ACT_GELU_TANH) return g * ffn_sigmoid(gelu_tanh_arg2(g));
+  else if constexpr (ACT == SBAMD_ACT_GELU) {
+    float phi, bell;
+    normal_parts(g, phi, bell);
+    return g * phi;
+  } else if constexpr (ACT == SBAMD_ACT_GELU_TANH) return g * ffn_sigmoid(gelu_tanh_arg2(g));
   else return g <= 0.0f ? 0.0f : g;  // NaN stays NaN
 }
 
@@ -112,9 +136,10 @@ __device__ inline void act_value_slope(float g, float& value, float& slope) {
     value = g * s;
     slope = s + value * (1.0f - s);
   } else if constexpr (ACT == SBAMD_ACT_GELU) {
-    const float phi = 0.5f * erfcf(-0.70710678118654752f * g);
+    float phi, bell;
+    normal_parts(g, phi, bell);
     value = g * phi;
-    slope = phi + g * 0.3989422804014327f * ffn_exp(-0.5f * g * g);
+    slope = phi + g * 0.3989422804014327f * bell;
   } else if constexpr (ACT == SBAMD_ACT_GELU_TANH) {
     // value = g s(z), z = 2 sqrt(2/pi) (g + 0.044715 g^3); slope = s + g s (1 - s) z'.  Far out s (1 - s) is 0
     // and z' is not: the product is taken only where s (1 - s) is not 0 (0 * inf would be NaN).

@@ -106,7 +106,7 @@ struct RingPlan {
 // bytes, and a matrix instruction takes the same time for either.  Measured on MI355X over n = 16 ... 21504, (k, m) = (1024, 4096),
 // (4096, 1024), (4096, 4096), (4096, 16384), (16384, 4096), plain and gated:
 //   128 x 128: 3.3e-3 us per byte of k with few tiles, 5.9e-3 with one per unit (8192 bytes: 33 / 51; 2048: 10 / 13.6), 6e-3 per
-//     tile and unit beyond (two share a unit, so no whole rounds: 448 tiles, 16384 bytes: 160); operands at 4.4 TB/s;
+//     tile and unit beyond (two share a unit, so no whole rounds: 448 tiles, 16384 bytes: 160); operands at 4.2 TB/s;
 //   256 x 256: 6 us and 13e-3 per byte and round of one tile per unit (2048 bytes, 10.5 rounds: 354; 8192: 1196), 8.2e-3
 //     with few units busy.
 // A tile count that leaves units idle in the last round (128 or 336 tiles of 256 x 256 on 256 units) has that round's tiles cut
@@ -123,7 +123,7 @@ RingPlan plan_ring(int64_t rows, int64_t n, int64_t len, int cus, bool cut) {
   const int64_t rounds = EDGE == 256 ? tiles / cus : 0, rest = tiles - rounds * cus;
   const double t_whole = 3.0 + double(rounds) * (6.0 + bytes * 13e-3);
   best.time = EDGE == 128 && q > 1.0 ? 3.0 + q * (bytes * 6.0e-3 + 0.7) : t_whole + (rest ? one_round(double(rest) / cus, bytes) : 0.0);
-  best.time = std::max(best.time, 3.0 + double(rows + n) * bytes / 4.4e6);
+  best.time = std::max(best.time, 3.0 + double(rows + n) * bytes / 4.2e6);
   constexpr int64_t SHORTEST = 8 * RING_BK;  // a slab, in 16-bit units: below that its prologue costs more than its work
   if (!cut || rest == 0 || k < 2 * SHORTEST || tiles > 0x7fff0000LL) return best;
   for (int64_t s = 2; s <= 32 && s * rest <= cus; ++s) {
@@ -137,8 +137,8 @@ RingPlan plan_ring(int64_t rows, int64_t n, int64_t len, int cus, bool cut) {
 }
 
 // The narrow kernel: operands at 6.2 TB/s; what the workgroups (32 rows x up to 64 tokens) read again through L2 at 28 TB/s, 12
-// where the tokens outgrow an XCD's 4 MB of it, both at 0.6 of that where rows are not 16-byte aligned; 3 us for each further
-// round of 512 workgroups (4550 of them with 64 bytes of k: 56); 1.2e-3 us per byte of k for a workgroup alone (rows 32768,
+// where the tokens outgrow an XCD's 4 MB of it, both at 0.6 of that where rows are not 16-byte aligned; 2 us for each further
+// round of 512 workgroups; 1.2e-3 us per byte of k for a workgroup alone (rows 32768,
 // 8192 bytes: n = 16 45 us, 48 58, 128 102; rows 8192: n = 224 43, 512 91).
 inline double narrow_time(int64_t rows, int64_t n, int64_t len, bool aligned) {
   const double b = double(len);
@@ -146,7 +146,7 @@ inline double narrow_time(int64_t rows, int64_t n, int64_t len, bool aligned) {
   const double blocks = double(ceil_div(n, tok)), wgs = double(ceil_div(rows, NARROW_ROWS)) * blocks;
   const double again = (wgs * double(tok) + (blocks - 1.0) * double(rows)) * b;
   const double moved = double(rows + n) * b / 6.2e6 + again / (double(n) * b <= 4.5e6 ? 28e6 : 12e6);
-  return 4.0 + std::max(b * 1.2e-3, aligned ? moved : moved / 0.6) + 3.0 * std::max(0.0, wgs / 512.0 - 1.0);
+  return 4.0 + std::max(b * 1.2e-3, aligned ? moved : moved / 0.6) + 2.0 * std::max(0.0, wgs / 512.0 - 1.0);
 }
 
 // One ring launch by its plan, and the join of what it cut.  g has operands, sizes and outputs set.

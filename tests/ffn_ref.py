@@ -88,11 +88,12 @@ def steep(g, kind):
 
 def act_error(g, kind):
     """Bound of |float act(g) - act(g)| for an exact g.  A handful of roundings of 2^-23 (the hardware's 2^x and
-    reciprocal are good to one unit in the last place, erfc of the device library to 16), and the argument's own
-    roundings (at most 6 of them) times the magnification."""
+    reciprocal are good to one unit in the last place, the polynomial behind Phi to 4e-7), and the argument's own
+    roundings (at most 6 of them) times the magnification.  The reciprocal and the exponential have no subnormal results: a
+    factor below 2^-126 becomes 0, and act(g), g times that factor, is then off by up to |g| 2^-126."""
     if kind == "relu":
         return np.zeros_like(g)
-    return np.abs(act(g, kind)) * (20.0 + 6.0 * steep(g, kind)) * 2.0 ** -23 + 2.0 ** -126
+    return np.abs(act(g, kind)) * (20.0 + 6.0 * steep(g, kind)) * 2.0 ** -23 + (1.0 + np.abs(g)) * 2.0 ** -126
 
 
 def slope_error(g, kind):

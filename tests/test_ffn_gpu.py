@@ -366,6 +366,20 @@ def test_gated_scaled_activations(h, out, kind):
     run_gated_scaled(h, out, 35, 70, 96, kind, scales=kind != "relu")
 
 
+@pytest.mark.parametrize("kind", ref.ACTS)
+def test_activation_over_its_whole_range(h, kind):
+    """act(g) in float for g from -12 to 12 and far beyond: k = 1, the gate's sum is an integer and its scale makes g, the other
+    half is 1.  Elementwise inside the relative bound, small values far on the negative side included."""
+    steps = np.concatenate([np.linspace(-12.0, 12.0, 4001), np.linspace(-60.0, 60.0, 95)]).astype(np.float32)
+    m = steps.size
+    x, w = np.ones((1, 1), np.int8), np.ones((2 * m, 1), np.int8)
+    xg, wg, c = Mat(h, "int8", 1, 1, values=x), Mat(h, "int8", 2 * m, 1, values=w), Mat(h, "float32", 1, m)
+    swg = vec(h, np.concatenate([steps, np.ones(m, np.float32)]))
+    h.wait(sb._gated_gemm_scaled(h, activation_t[kind], "t", "n", m, 1, 1, wg.buf, 1, swg.buf, xg.buf, 1, None, c.buf, m))
+    g = steps.astype(np.float64)[None, :]
+    close(c.get().astype(np.float64), ref.act(g, kind), ref.act_error(g, kind) + 2 * ref.U32 * np.abs(ref.act(g, kind)), kind)
+
+
 @pytest.mark.parametrize("ta,tb", [("t", "n"), ("n", "n"), ("t", "t"), ("n", "t")])
 @pytest.mark.parametrize("n,m,k,pad,shift", [(5, 40, 70, 0, 0), (40, 96, 200, 3, 1), (136, 264, 96, 16, 0)])
 def test_gated_scaled_layouts(h, ta, tb, n, m, k, pad, shift):
