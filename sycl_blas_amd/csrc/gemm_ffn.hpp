@@ -401,6 +401,8 @@ __global__ void __launch_bounds__(NARROW_WAVES * 64, OCC) ffn_narrow_kernel(cons
 // bytes], 16-byte piece c of row r at c ^ ((r >> 1) & 7)) and leave as whole rows of up to 128 bytes (element by element where
 // C's rows are not 16-byte aligned or the tile hangs over the edge).  16-bit results are rounded on the way into the
 // corner; with beta * C to add they stay float there and are rounded once behind the addition.
+// Bands of four tile rows instead of the GEMM's eight: 8-bit gated 1712 x 4096 -> 16384 229 -> 224 us, the rest within 1 %.
+constexpr int RING_BAND = 4;
 constexpr int CORNER_ROW = 128, CORNER_BYTES = 32 * CORNER_ROW;
 __device__ inline int corner_at(int row, int byte) { return row * CORNER_ROW + (((byte >> 4) ^ ((row >> 1) & 7)) << 4) + (byte & 15); }
 
@@ -511,7 +513,7 @@ __global__ void __launch_bounds__(WM* WN * 64, 2) ffn_ring_kernel(const FfnArgs<
       a += TA ? k0 : k0 * lda;
       b += TB ? k0 * ldb : k0;
     }
-    tile_coords(tile, g.tiles_m, g.tiles_n, tm, tn);
+    tile_coords(tile, g.tiles_m, g.tiles_n, tm, tn, BM == 256 ? RING_BAND : 0);
     m0 = int64_t(tm) * CHB, n0 = int64_t(tn) * BN;
     if constexpr (GATED) oa.init_gated(a, lda, m0, g.m, tid);
     else oa.init(a, lda, m0, g.m, tid);
@@ -536,7 +538,7 @@ __global__ void __launch_bounds__(WM* WN * 64, 2) ffn_ring_kernel(const FfnArgs<
 
   // vector stores of a whole tile's epilogue, per wavefront
   constexpr int STORES = NI * 32 * CHW * int(sizeof(TOut)) / 1024;
-  bool stored = false;  // the last epilogue issued exactly STORES of them behind the loads of the tile to come
+  bool stored = false;  // the last epilogue issued at least that many behind the loads of the tile to come
   begin(blockIdx.x);
   for (int unit = blockIdx.x;;) {
     Acc acc[MI][NI];
@@ -670,7 +672,7 @@ __global__ void __launch_bounds__(WM* WN * 64, 2) ffn_ring_kernel(const FfnArgs<
         static_for<NI>([&](auto j) __attribute__((always_inline)) { emit(as_float{}, j, scaled, g.c, g.ldc, vec_c, true); });
       }
     }
-    // (with P kept there are more stores than that: waiting for fewer is then merely early)
+    // (with P kept there are more stores than that: the wait is then merely earlier than it need be)
     stored = vec_c && !partial && (GATED || g.beta_zero) && ch0 + CHW <= g.m && tok0 + WTN <= g.n;
     if (next >= units) return;
     unit = next;
@@ -687,7 +689,7 @@ __global__ void __launch_bounds__(256) ffn_join_kernel(const FfnArgs<TOut> g) {
   constexpr int PER_TILE = BM * BN / 8;
   const int t = int(v / PER_TILE), at = int(v % PER_TILE) * 8;  // (the grid is whole tiles)
   int tm, tn;
-  tile_coords(g.whole + t, g.tiles_m, g.tiles_n, tm, tn);
+  tile_coords(g.whole + t, g.tiles_m, g.tiles_n, tm, tn, BM == 256 ? RING_BAND : 0);
   const int64_t ch = int64_t(tm) * BM + at % BM, tok = int64_t(tn) * BN + at / BM;
   if (ch >= g.m || tok >= g.n) return;
   const Sum* src = static_cast<const Sum*>(g.cube) + int64_t(t) * g.slabs * (BM * BN) + at;

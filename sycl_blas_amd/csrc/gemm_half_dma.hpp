@@ -206,7 +206,7 @@ struct RingOperand {
 // acc += (the tile of op(A)) * (the tile of op(B)) over k_len, the operands' pointers set up by init: the ring itself.
 // M_FIRST: a lane ends up with one index of A (lane & 31) and sixteen of B, else the other way round.
 // STAGES - 1 tiles are kept in flight.  STARTED: the first ones are on their way already (ring_start), and `stores` says that
-// exactly STORES vector stores (and nothing else) were issued behind them: memory operations complete in order, so the first
+// at least STORES vector stores were issued behind them: memory operations complete in order, so the first
 // tiles are waited for without waiting for those stores.
 template <typename Tag, typename OpA, typename OpB, int MI, int NI, int WTM, int WTN, int ABLATE, bool M_FIRST, int STAGES, bool STARTED, int STORES = 0, typename Acc>
 __device__ __attribute__((always_inline)) inline void ring_multiply(Acc (&acc)[MI][NI], OpA& oa, OpB& ob, const int64_t lda, const int64_t ldb,
