@@ -13,6 +13,13 @@
  * the other transposes work too, some of them through a repacked copy of the
  * operand in the handle's own scratch area.
  *
+ * Scratch and graphs: repacked operands and products cut along k use scratch areas of the handle, which grow
+ * at the first call that needs them; such a call has to have run once before it is captured, and graphs captured
+ * from one handle share the areas, so they must not replay at the same time.
+ *
+ * sbamd_set_kernel pins SBAMD_KERNEL_SMALL (few tokens), _LARGE (128 x 128 tiles) or _HUGE (256 x 256);
+ * sbamd_last_kernel and sbamd_last_splitk report what ran.
+ *
  * Every leading dimension must be at least the number of rows of its matrix.
  * Outputs must not overlap inputs unless an entry point says so.
  *

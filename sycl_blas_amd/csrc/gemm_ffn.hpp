@@ -99,7 +99,7 @@ __device__ inline float gelu_tanh_arg2(float g) { return 1.5957691216057308f * (
 // Phi(g) and e^(-g^2/2), one exponential for both: with x = |g| / sqrt(2), erfc(x) = e^(-x^2) R(x), and R is a polynomial in
 // t = 1 / (1 + 0.4 x), fitted for the least largest relative error over 0 <= x <= 9.5 (8.4e-8; 4.3e-7 as evaluated in float), so the
 // small values of Phi far on the negative side keep their relative precision, which 1 + erf would cancel away.
-// (The device library's erfc took two thirds of the elementwise gradient's time for this activation.)
+// (With the device library's erfc the elementwise gradient took 11.8 us at 1119 x 2730, so 8.5.)
 __device__ inline void normal_parts(float g, float& phi, float& bell) {
   const float x = __builtin_fabsf(g) * 0.70710678118654752f;
   const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.4f, x, 1.0f));

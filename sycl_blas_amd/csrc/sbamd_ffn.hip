@@ -417,7 +417,7 @@ int gradient(sbamd_handle_t hh, int act, char transa, char transb, int64_t m, in
   };
   const bool want_a = da && m > 0 && k > 0, want_b = db && n > 0 && k > 0;
   // A dP whose rows do not come in whole 16-byte pieces keeps the ring from reading it (2 * 2730 rows, 1119 tokens, k = 1000:
-  // 47 us for dA against 29): the elementwise pass then writes a second, padded one into the handle's scratch area.
+  // 47 us for dA where the padded copy takes 29; later steps brought that to 25): the elementwise pass then writes a second, padded one into the handle's scratch area.
   uint16_t* copy = nullptr;
   const int64_t ld_copy = ceil_div(2 * m, 8) * 8;
   if (tokens && h->kernel_override != SBAMD_KERNEL_SMALL) {
@@ -438,18 +438,18 @@ int gradient(sbamd_handle_t hh, int act, char transa, char transb, int64_t m, in
     if (e != hipSuccess) return ffn_fail(h, e, "gradient launch");
   }
   // The products run with n (m) == 0 too: a sum over nothing is beta times what was there.
-  if (want_a) {
-    Product<TOut> q = product_a(dp, lddp, 0);
-    if (copy && !ring_reads_product(q) && ring_reads_product(product_a(copy, ld_copy, ld_copy))) q = product_a(copy, ld_copy, ld_copy);
-    const hipError_t e = run_product<Tag, TOut>(h, q);
-    if (e != hipSuccess) return ffn_fail(h, e, "gradient product");
-  }
-  if (want_b) {
-    Product<TOut> q = product_b(dp, lddp);
-    if (copy && !ring_reads_product(q) && ring_reads_product(product_b(copy, ld_copy))) q = product_b(copy, ld_copy);
-    const hipError_t e = run_product<Tag, TOut>(h, q);
-    if (e != hipSuccess) return ffn_fail(h, e, "gradient product");
-  }
+  Product<TOut> qa = product_a(dp, lddp, 0), qb = product_b(dp, lddp);
+  const bool copy_a = copy && want_a && !ring_reads_product(qa) && ring_reads_product(product_a(copy, ld_copy, ld_copy));
+  const bool copy_b = copy && want_b && !ring_reads_product(qb) && ring_reads_product(product_b(copy, ld_copy));
+  if (copy_a) qa = product_a(copy, ld_copy, ld_copy);
+  if (copy_b) qb = product_b(copy, ld_copy);
+  // A product the ring does not take may repack its operands into the scratch area that the copy is in, or have
+  // it replaced by a larger one: whichever reads the copy goes first.
+  hipError_t e = hipSuccess;
+  if (copy_b && !copy_a) e = run_product<Tag, TOut>(h, qb);
+  if (e == hipSuccess && want_a) e = run_product<Tag, TOut>(h, qa);
+  if (e == hipSuccess && want_b && !(copy_b && !copy_a)) e = run_product<Tag, TOut>(h, qb);
+  if (e != hipSuccess) return ffn_fail(h, e, "gradient product");
   return SBAMD_OK;
 }
 

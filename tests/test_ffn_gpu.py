@@ -387,7 +387,8 @@ def test_gated_scaled_layouts(h, ta, tb, n, m, k, pad, shift):
 
 
 # ------------------------------------------------------------------- gradient
-def run_grad(h, dtype, n, m, k, kind, ta="t", tb="n", pad=0, shift=0, beta_a=0.0, beta_b=0.0, in_place=False, want="ab", family=AUTO):
+def run_grad(h, dtype, n, m, k, kind, ta="t", tb="n", pad=0, shift=0, beta_a=0.0, beta_b=0.0, in_place=False, want="ab", family=AUTO,
+             pad_w=None, pad_x=None):
     rng = seeded("grad", dtype, n, m, k, kind, ta, tb, pad, shift, beta_a, beta_b, in_place, want)
     xb, x = ref.to_bits(rng.standard_normal((n, k)), dtype)
     wb, w = ref.to_bits(rng.standard_normal((2 * m, k)) / math.sqrt(max(k, 1)), dtype)
@@ -396,11 +397,13 @@ def run_grad(h, dtype, n, m, k, kind, ta="t", tb="n", pad=0, shift=0, beta_a=0.0
     daw, da0 = ref.to_bits(rng.standard_normal((2 * m, k)), dtype)
     dbx, db0 = ref.to_bits(rng.standard_normal((n, k)), dtype)
 
+    pad_w, pad_x = pad if pad_w is None else pad_w, pad if pad_x is None else pad_x
+
     def weights(values):
-        return Mat(h, dtype, 2 * m, k, k + pad, shift, values) if ta == "t" else Mat(h, dtype, k, 2 * m, 2 * m + pad, shift, across(values))
+        return Mat(h, dtype, 2 * m, k, k + pad_w, shift, values) if ta == "t" else Mat(h, dtype, k, 2 * m, 2 * m + pad_w, shift, across(values))
 
     def tokens(values):
-        return Mat(h, dtype, n, k, k + pad, shift, values) if tb == "n" else Mat(h, dtype, k, n, n + pad, shift, across(values))
+        return Mat(h, dtype, n, k, k + pad_x, shift, values) if tb == "n" else Mat(h, dtype, k, n, n + pad_x, shift, across(values))
 
     wg, xg = weights(wb), tokens(xb)
     pg = Mat(h, dtype, n, 2 * m, 2 * m + pad, shift, pb)
@@ -465,6 +468,21 @@ def test_grad_families(h, family, n, m, k, ta, tb):
     channels and 2500 tokens leave rows that do not come in whole 16-byte pieces."""
     run_grad(h, "bfloat16", n, m, k, "silu", ta, tb, beta_a=0.5 if m > 100 else 0.0, family=FAMILIES[family])
     run_grad(h, "float16", n, m, k, "gelu_tanh", ta, tb, pad=8, beta_b=1.0 if m > 100 else 0.0, family=FAMILIES[family])
+
+
+@pytest.mark.parametrize("pad_w,pad_x", [(0, 3), (3, 0), (3, 3)])
+@pytest.mark.parametrize("ta,tb", [("t", "n"), ("n", "n"), ("t", "t")])
+@pytest.mark.parametrize("n,m,k", [(200, 34, 72), (1104, 302, 136)])
+def test_grad_products_share_the_scratch_area(h, n, m, k, ta, tb, pad_w, pad_x):
+    """dP's rows are not whole 16-byte pieces, so one product reads a padded copy of it in the handle's scratch area, while
+    the other, whose second operand is misaligned, has both of its operands repacked into the same area (parameter bit 0 of the
+    16-bit back end asks for that at any size): neither may take the other's place.  Twice, with the area grown the second time."""
+    own = sb.SB_Handle(0)
+    try:
+        for tokens in (n // 2 // 8 * 8, n, n):
+            run_grad(own, "bfloat16", tokens, m, k, "silu", ta, tb, family=(_lib.KERNEL_AUTO, 1), pad_w=pad_w, pad_x=pad_x)
+    finally:
+        own.close()
 
 
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
