@@ -955,9 +955,15 @@ __global__ void __launch_bounds__(256)
   auto one = [&](uint16_t gb, uint16_t ub, uint16_t db, uint16_t& dg, uint16_t& du) {
     float value, slope;
     act_value_slope<decltype(act_tag)::value>(widen(Tag{}, gb), value, slope);
-    const float d = widen(Tag{}, db);
+    const float d = widen(Tag{}, db), u = widen(Tag{}, ub);
+    // d u may pass the float range where a small slope brings the product back (0 times the infinity would be NaN); the
+    // slope goes first there: with |d u| >= 2^128 both are above 1, so nothing underflows that the slope itself kept
+    float du_slope = d * u * slope;
+    if constexpr (std::is_same<Tag, Bf16Tag>::value) {  // (two halves stay below 2^32)
+      if (__builtin_fabsf(d * u) > 3.4028234663852886e38f) du_slope = d * slope * u;
+    }
     TOut og, ou;
-    store_out(&og, d * widen(Tag{}, ub) * slope);
+    store_out(&og, du_slope);
     store_out(&ou, d * value);
     dg = __builtin_bit_cast(uint16_t, og);
     du = __builtin_bit_cast(uint16_t, ou);

@@ -513,6 +513,29 @@ def test_grad_far_out(h, kind):
     close(got, dp, bound + 2.0 ** -24, f"far {kind}")
 
 
+@pytest.mark.parametrize("kind", ref.ACTS)
+def test_grad_of_products_beyond_float(h, kind):
+    """bfloat16 dC and U whose product no float holds, under slopes that are 0 or small: the infinity must not meet the slope."""
+    gates = np.array([-200.0, -40.0, -1e30, 0.0, -60.0, -0.0, 3.0, -25.0])
+    m, n = len(gates), 3
+    u = np.array([1e20, -3e30, 2e38])[:, None] * np.ones((n, m))
+    pb, p = ref.to_bits(np.concatenate([np.tile(gates, (n, 1)), u], 1), "bfloat16")
+    db, dh = ref.to_bits(np.array([3e18, 2e20, -1e10])[:, None] * np.ones((n, m)), "bfloat16")
+    pg, dcg, dpg = Mat(h, "bfloat16", n, 2 * m, values=pb), Mat(h, "bfloat16", n, m, values=db), Mat(h, "bfloat16", n, 2 * m)
+    h.wait(sb._gated_gemm_grad(h, activation_t[kind], "t", "n", m, n, 1, None, 0, None, 0, pg.buf, 2 * m, dcg.buf, m, dpg.buf, 2 * m,
+                               0.0, None, 0, 0.0, None, 0))
+    got = ref.from_bits(dpg.get(), "bfloat16")
+    assert not np.isnan(got).any()
+    with np.errstate(all="ignore"):
+        s = np.where(np.abs(p[:, :m]) < 1e10, ref.slope(np.clip(p[:, :m], -1e10, 1e10), kind), 0.0)  # (all four are 0 at -1e30)
+    dg = dh * p[:, m:] * np.nan_to_num(s)
+    for i, j in np.ndindex(n, m):
+        if s[i, j] == 0:
+            assert got[i, j] == 0, (kind, i, j)
+        elif abs(s[i, j]) > 0.1:  # the slope is accurate there: in range it has to be right, beyond it an infinity
+            assert np.isinf(got[i, j]) if abs(dg[i, j]) > 3.5e38 else abs(got[i, j] / dg[i, j] - 1) < 2.0 ** -7, (kind, i, j)
+
+
 def test_grad_of_no_tokens_scales_what_is_there(h):
     m, k = 12, 20
     rng = seeded("no tokens")
