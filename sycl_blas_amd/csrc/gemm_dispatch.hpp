@@ -778,8 +778,8 @@ hipError_t run_scale_real(Handle* h, T* c, int64_t rows, int64_t cols, int64_t l
   const int64_t total = rows * cols * batch;
   if (total <= 0) return hipSuccess;
   const int64_t grid = ceil_div(total, 256);
-  if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((scale_matrix_kernel<T>), dim3((unsigned)grid), dim3(256), 0, h->stream, c,
+  if (grid > MAX_GRID) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((scale_matrix_kernel<T>), folded_grid(grid, 256), dim3(256), 0, h->stream, c,
                      rows, cols, ld, stride, batch, beta, assign_zero ? 1 : 0);
   return hipGetLastError();
 }

@@ -230,7 +230,10 @@ __global__ void __launch_bounds__(NARROW_WAVES * 64, OCC) ffn_narrow_kernel(cons
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int logical = xcd_remap(blockIdx.x, gridDim.x);
+  const int64_t block = folded_block();
+  const int blocks = g.tiles_m * g.tiles_n;
+  if (block >= blocks) return;
+  const int logical = xcd_remap(int(block), blocks);
   const int tm = logical / g.tiles_n, tn = logical - tm * g.tiles_n;  // the token blocks of one row block are neighbours
   const int64_t m0 = int64_t(tm) * CH, n0 = int64_t(tn) * TOK;
 
@@ -739,7 +742,7 @@ template <int BYTES>
 __global__ void __launch_bounds__(256)
     ffn_pack_rows_kernel(const unsigned char* __restrict__ src, int64_t ld, unsigned char* __restrict__ dst, int64_t row_bytes, int64_t rows,
                          int64_t k) {
-  const int64_t per = row_bytes / 16, v = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t per = row_bytes / 16, v = folded_block() * 256 + threadIdx.x;
   if (v >= per * rows) return;
   const int64_t r = v / per, at = (v - r * per) * 16, kb = k * BYTES;
   const unsigned char* s = src + r * ld * BYTES + at;
@@ -760,7 +763,7 @@ __global__ void __launch_bounds__(256)
   typedef uint32_t u32_at1 __attribute__((aligned(1)));
   __shared__ uint32_t tile[ROWS * PITCH / 4];
   const int64_t k_tiles = (row_bytes + PACK_K_BYTES - 1) / PACK_K_BYTES;
-  const int64_t r0 = int64_t(blockIdx.x) / k_tiles * ROWS, k0 = int64_t(blockIdx.x) % k_tiles * KS;
+  const int64_t r0 = folded_block() / k_tiles * ROWS, k0 = folded_block() % k_tiles * KS;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t r = r0 + lane * U;
   uint32_t in[KS / U / 4][U];
@@ -860,7 +863,7 @@ __global__ void __launch_bounds__(TPC < 256 ? 256 : TPC)
   constexpr int COLS = TPC < 256 ? 256 / TPC : 1;
   typedef uint32_t u32x2_at1 __attribute__((ext_vector_type(2), aligned(1)));
   const int t = threadIdx.x % TPC;
-  const int64_t col = int64_t(blockIdx.x) * COLS + threadIdx.x / TPC;
+  const int64_t col = folded_block() * COLS + threadIdx.x / TPC;
   const bool live = col < n;  // (whole wavefronts are live or not)
   const typename In::type* src = x + (live ? col : n - 1) * ldx;
   const int64_t vecs = m / 8;
@@ -944,7 +947,7 @@ __global__ void __launch_bounds__(256)
     ffn_gate_grad_kernel(int act, int64_t m, int64_t n, const uint16_t* p, int64_t ldp, const uint16_t* dc, int64_t lddc, uint16_t* dp,
                          int64_t lddp, uint16_t* copy, int64_t ld_copy) {
   const int64_t per = (m + 7) / 8;
-  const int64_t v = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t v = folded_block() * 256 + threadIdx.x;
   if (v >= per * n) return;
   const int64_t col = v / per, i = (v - col * per) * 8;
   const uint16_t* pg = p + col * ldp + i;

@@ -513,7 +513,7 @@ static __global__ void __launch_bounds__(256)
     scale_matrix16_kernel(uint16_t* c, int64_t rows, int64_t cols, int64_t ld, int64_t stride, int64_t batch,
                           float beta, int assign_zero) {
   const int64_t per = rows * cols;
-  const int64_t gid = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t gid = folded_block() * 256 + threadIdx.x;
   if (gid >= per * batch) return;
   const int64_t z = gid / per;
   const int64_t idx = gid - z * per;

@@ -345,6 +345,16 @@ __device__ inline int xcd_remap(int bid, int nwg) {
   return base + (bid >> 3);
 }
 
+// A launch holds fewer than 2^32 threads along x.  A longer list of workgroups is folded into rows of equal length along y;
+// fewer workgroups than there are rows are left over at the end and have to find nothing to do.
+constexpr int64_t MAX_GRID = int64_t(65535) << 20;  // workgroups a folded launch can hold
+inline dim3 folded_grid(int64_t blocks, int threads) {
+  if (blocks * threads < (int64_t(1) << 32)) return dim3((unsigned)blocks);
+  const int64_t rows = (blocks + (int64_t(1) << 20) - 1) >> 20;
+  return dim3((unsigned)((blocks + rows - 1) / rows), (unsigned)rows);
+}
+__device__ inline int64_t folded_block() { return int64_t(blockIdx.y) * gridDim.x + blockIdx.x; }
+
 // Rows of tiles are walked in bands of GROUP_M so that a run of consecutive
 // logical ids touches few distinct A and B panels.
 // The 32 workgroups resident on one XCD (one per compute unit) then form a GROUP_M x 32/GROUP_M patch
@@ -2117,7 +2127,7 @@ __global__ void __launch_bounds__(256)
     scale_matrix_kernel(T* c, int64_t rows, int64_t cols, int64_t ld, int64_t stride,
                         int64_t batch, T beta, int assign_zero) {
   const int64_t per = rows * cols;
-  const int64_t gid = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t gid = folded_block() * 256 + threadIdx.x;
   if (gid >= per * batch) return;
   const int64_t z = gid / per;
   const int64_t idx = gid - z * per;

@@ -39,7 +39,7 @@ hipError_t launch_narrow(FfnArgs<TOut> g, hipStream_t stream) {
   if (tm > 0x7fffffffLL / tn) return hipErrorInvalidValue;
   g.tiles_m = int32_t(tm);
   g.tiles_n = int32_t(tn);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(NARROW_WAVES * 64), lds, stream, g);
+  hipLaunchKernelGGL(kernel, folded_grid(tm * tn, NARROW_WAVES * 64), dim3(NARROW_WAVES * 64), lds, stream, g);
   return hipGetLastError();
 }
 
@@ -55,11 +55,11 @@ template <int BYTES>
 hipError_t pack(Handle* h, const Rows& o, unsigned char* dst, int64_t row_bytes) {
   const unsigned char* src = static_cast<const unsigned char*>(o.x);
   const int64_t grid = o.across ? ceil_div(o.rows, PACK_R_BYTES / BYTES) * ceil_div(row_bytes, PACK_K_BYTES) : ceil_div(row_bytes / 16 * o.rows, 256);
-  if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
+  if (grid > MAX_GRID) return hipErrorInvalidValue;
   if (o.across)
-    hipLaunchKernelGGL((ffn_pack_across_kernel<BYTES>), dim3((unsigned)grid), dim3(256), 0, h->stream, src, o.ld, dst, row_bytes, o.rows, o.k);
+    hipLaunchKernelGGL((ffn_pack_across_kernel<BYTES>), folded_grid(grid, 256), dim3(256), 0, h->stream, src, o.ld, dst, row_bytes, o.rows, o.k);
   else
-    hipLaunchKernelGGL((ffn_pack_rows_kernel<BYTES>), dim3((unsigned)grid), dim3(256), 0, h->stream, src, o.ld, dst, row_bytes, o.rows, o.k);
+    hipLaunchKernelGGL((ffn_pack_rows_kernel<BYTES>), folded_grid(grid, 256), dim3(256), 0, h->stream, src, o.ld, dst, row_bytes, o.rows, o.k);
   return hipGetLastError();
 }
 
@@ -238,7 +238,7 @@ hipError_t scale_c<uint16_t>(Handle* h, uint16_t* c, int64_t m, int64_t n, int64
   return run_scale_f16(h, c, m, n, ldc, 0, 1, beta, beta == 0.0f);
 }
 __global__ void __launch_bounds__(256) ffn_scale_bf16_kernel(bf16_bits* c, int64_t m, int64_t n, int64_t ldc, float beta, int beta_zero) {
-  const int64_t idx = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t idx = folded_block() * 256 + threadIdx.x;
   if (idx >= m * n) return;
   bf16_bits* p = c + idx % m + idx / m * ldc;
   store_out(p, beta_zero ? 0.0f : beta * load_out(p));
@@ -246,8 +246,8 @@ __global__ void __launch_bounds__(256) ffn_scale_bf16_kernel(bf16_bits* c, int64
 template <>
 hipError_t scale_c<bf16_bits>(Handle* h, bf16_bits* c, int64_t m, int64_t n, int64_t ldc, float beta) {
   const int64_t grid = ceil_div(m * n, 256);
-  if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(ffn_scale_bf16_kernel, dim3((unsigned)grid), dim3(256), 0, h->stream, c, m, n, ldc, beta, beta == 0.0f ? 1 : 0);
+  if (grid > MAX_GRID) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(ffn_scale_bf16_kernel, folded_grid(grid, 256), dim3(256), 0, h->stream, c, m, n, ldc, beta, beta == 0.0f ? 1 : 0);
   return hipGetLastError();
 }
 
@@ -304,10 +304,10 @@ int forward(sbamd_handle_t hh, int act, char transa, char transb, int64_t m, int
 template <typename Tag, int TPC, int HOLD>
 hipError_t launch_quantize(Handle* h, int64_t m, int64_t n, const typename QuantIn<Tag>::type* x, int64_t ldx, int8_t* q, int64_t ldq,
                            float* scale) {
-  constexpr int COLS = TPC < 256 ? 256 / TPC : 1;
+  constexpr int COLS = TPC < 256 ? 256 / TPC : 1, THREADS = TPC < 256 ? 256 : TPC;
   const int64_t grid = ceil_div(n, COLS);
-  if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((ffn_quantize_kernel<Tag, TPC, HOLD>), dim3((unsigned)grid), dim3(TPC < 256 ? 256 : TPC), 0, h->stream, m, n, x, ldx, q,
+  if (grid > MAX_GRID) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((ffn_quantize_kernel<Tag, TPC, HOLD>), folded_grid(grid, THREADS), dim3(THREADS), 0, h->stream, m, n, x, ldx, q,
                      ldq, scale);
   return hipGetLastError();
 }
@@ -418,6 +418,8 @@ int gradient(sbamd_handle_t hh, int act, char transa, char transb, int64_t m, in
   const bool want_a = da && m > 0 && k > 0, want_b = db && n > 0 && k > 0;
   // A dP whose rows do not come in whole 16-byte pieces keeps the ring from reading it (2 * 2730 rows, 1119 tokens, k = 1000:
   // 47 us for dA where the padded copy takes 29; later steps brought that to 25): the elementwise pass then writes a second, padded one into the handle's scratch area.
+  const int64_t grid = ceil_div(ceil_div(m, 8) * n, 256);
+  if (grid > MAX_GRID) return SBAMD_INVALID_VALUE;
   uint16_t* copy = nullptr;
   const int64_t ld_copy = ceil_div(2 * m, 8) * 8;
   if (tokens && h->kernel_override != SBAMD_KERNEL_SMALL) {
@@ -430,9 +432,7 @@ int gradient(sbamd_handle_t hh, int act, char transa, char transb, int64_t m, in
     }
   }
   if (tokens) {
-    const int64_t grid = ceil_div(ceil_div(m, 8) * n, 256);
-    if (grid > 0x7fffffffLL) return SBAMD_INVALID_VALUE;
-    hipLaunchKernelGGL((ffn_gate_grad_kernel<Tag, TOut>), dim3((unsigned)grid), dim3(256), 0, h->stream, act, m, n, p, ldp, dc, lddc, dp, lddp, copy,
+    hipLaunchKernelGGL((ffn_gate_grad_kernel<Tag, TOut>), folded_grid(grid, 256), dim3(256), 0, h->stream, act, m, n, p, ldp, dc, lddc, dp, lddp, copy,
                        ld_copy);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return ffn_fail(h, e, "gradient launch");

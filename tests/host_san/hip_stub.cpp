@@ -20,6 +20,7 @@ std::map<uintptr_t, size_t> g_allocs;          // base -> bytes
 std::map<const void*, size_t> g_symbols;       // host stand-in of a device variable -> bytes
 std::map<const void*, void*> g_symbol_memory;  // ... -> its "device" memory
 long g_launches = 0;
+uint64_t g_widest = 0;  // most threads along one axis of a launch since last asked
 int g_device = 0;
 struct Config {
   dim3 grid, block;
@@ -48,6 +49,11 @@ hipError_t alloc(void** p, size_t bytes) {
 }  // namespace
 
 extern "C" long hip_stub_launches() { return g_launches; }
+extern "C" uint64_t hip_stub_widest_launch() {
+  const uint64_t widest = g_widest;
+  g_widest = 0;
+  return widest;
+}
 extern "C" long hip_stub_live_allocations() {
   std::lock_guard<std::mutex> lock(g_mu);
   return long(g_allocs.size());
@@ -83,6 +89,8 @@ hipError_t hipLaunchKernel(const void* f, dim3 grid, dim3 block, void** args, si
                  block.x, block.y, block.z, lds);
     std::abort();
   }
+  for (const uint64_t along : {uint64_t(grid.x) * block.x, uint64_t(grid.y) * block.y, uint64_t(grid.z) * block.z})
+    if (along > g_widest) g_widest = along;
   ++g_launches;
   return hipSuccess;
 }
