@@ -18,7 +18,7 @@
  * from one handle share the areas, so they must not replay at the same time.
  *
  * sbamd_set_kernel pins SBAMD_KERNEL_SMALL (few tokens), _LARGE (128 x 128 tiles) or _HUGE (256 x 256);
- * sbamd_last_kernel and sbamd_last_splitk report what ran.
+ * sbamd_last_kernel and sbamd_last_splitk report what ran; after a gradient, its last product (-1 if it had none).
  *
  * Every leading dimension must be at least the number of rows of its matrix.
  * Outputs must not overlap inputs unless an entry point says so.

@@ -357,6 +357,7 @@ bool ring_reads_product(const Product<TOut>& q) {
 template <typename Tag, typename TOut>
 hipError_t run_product(Handle* h, const Product<TOut>& q) {
   const int cus = h->compute_units > 0 ? h->compute_units : 256;
+  h->last_depth = 1, h->last_k_chunk = q.k;  // (the gradient's other product may have been cut)
   if (ring_reads_product(q) && h->kernel_override != SBAMD_KERNEL_SMALL) {
     const RingPlan big = plan_ring<256>(q.m, q.n, 2 * q.k, cus, true), small = plan_ring<128>(q.m, q.n, 2 * q.k, cus, true);
     const bool take_big = h->kernel_override == SBAMD_KERNEL_HUGE || (h->kernel_override != SBAMD_KERNEL_LARGE && big.time < small.time);
