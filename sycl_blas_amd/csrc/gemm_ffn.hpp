@@ -536,7 +536,7 @@ __global__ void __launch_bounds__(WM* WN * 64, 2) ffn_ring_kernel(const FfnArgs<
         sb[j] = g.scale_b ? g.scale_b[t < g.n ? t : g.n - 1] : 1.0f;
       }
     }
-    ring_start<OpA, OpB, RING_STAGES>(oa, ob, lda, ldb, int(k_len / RING_BK), smem, wave);
+    ring_start(oa, ob, lda, ldb, int(k_len / RING_BK), smem, wave);
   };
 
   // vector stores of a whole tile's epilogue, per wavefront
@@ -552,7 +552,7 @@ __global__ void __launch_bounds__(WM* WN * 64, 2) ffn_ring_kernel(const FfnArgs<
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
     // (its first barrier lies behind every wavefront's epilogue of the tile before, so the last stage may be refilled)
-    ring_multiply<Tag, OpA, OpB, MI, NI, WTM, WTN, 0, false, RING_STAGES, true, STORES>(acc, oa, ob, lda, ldb, k_len, smem, tid, lane, wave, wm,
+    ring_multiply<Tag, OpA, OpB, MI, NI, WTM, WTN, 0, false, STORES>(acc, oa, ob, lda, ldb, k_len, smem, tid, lane, wave, wm,
                                                                                        wn, stored);
 
     __syncthreads();  // every wavefront is through with the ring's stages

@@ -53,7 +53,7 @@ typedef __attribute__((address_space(3))) void* dma_lptr_t;
 // fetched behind the remaining matrix instructions).
 constexpr int RING_BK = 32, RING_STAGES = 5, RING_AHEAD = 4;
 constexpr int ring_operand_bytes(int rows) { return rows * RING_BK * 2; }  // 256 rows: 16 KiB
-constexpr int ring_lds_bytes(int bm, int bn, int stages = RING_STAGES) { return stages * (ring_operand_bytes(bm) + ring_operand_bytes(bn)); }
+constexpr int ring_lds_bytes(int bm, int bn) { return RING_STAGES * (ring_operand_bytes(bm) + ring_operand_bytes(bn)); }
 constexpr int RING_LDS_BYTES = ring_lds_bytes(DMA_BM, DMA_BN);
 
 // Images per stage and operand (ROWS = 256 or 128 indices along M / N; 16 or 8 KiB):
@@ -201,202 +201,34 @@ struct RingOperand {
 
 };
 
-// ABLATE is a timing-only diagnostic (bit 1: no loads inside the K loop, bit 2: no matrix
-// instructions, bit 4: no fragment reads); the library instantiates 0.
-// acc += (the tile of op(A)) * (the tile of op(B)) over k_len, the operands' pointers set up by init: the ring itself.
-// M_FIRST: a lane ends up with one index of A (lane & 31) and sixteen of B, else the other way round.
-// STAGES - 1 tiles are kept in flight.  STARTED: the first ones are on their way already (ring_start), and `stores` says that
-// at least STORES vector stores were issued behind them: memory operations complete in order, so the first
-// tiles are waited for without waiting for those stores.
-template <typename Tag, typename OpA, typename OpB, int MI, int NI, int WTM, int WTN, int ABLATE, bool M_FIRST, int STAGES, bool STARTED, int STORES = 0, typename Acc>
-__device__ __attribute__((always_inline)) inline void ring_multiply(Acc (&acc)[MI][NI], OpA& oa, OpB& ob, const int64_t lda, const int64_t ldb,
-                                                                    const int64_t k_len, SBAMD_LDS unsigned char* smem, const int tid,
-                                                                    const int lane, const int wave, const int wm, const int wn, const bool stores = false) {
-  constexpr int NM = MI * NI;   // matrix instructions per half step
-  constexpr int NPA = OpA::NP, NPB = OpB::NP;    // load instructions per thread and tile of each operand
-  constexpr int LPA = NPA / 2, LPH = LPA + NPB / 2;  // of them per half step: A's, both operands'
-  constexpr int AHEAD = STAGES - 1;
-  constexpr int RING_OPERAND_BYTES = OpA::BYTES;  // offset of the B image inside a stage
-  constexpr int RING_STAGE_BYTES = OpA::BYTES + OpB::BYTES;
-  const int nk = int(k_len / RING_BK);
-
-  auto stage_ptr = [&](int t) { return smem + (t % STAGES) * RING_STAGE_BYTES; };
-
-  if constexpr (!STARTED) {
-    // prologue: tiles 0 .. AHEAD-1 (those that exist) go in flight
-#pragma unroll
-    for (int t = 0; t < AHEAD; ++t) {
-      if (t < nk) {
-        SBAMD_LDS unsigned char* st = smem + t * RING_STAGE_BYTES;
-        static_for<NPA>([&](auto i) { oa.template issue_piece<decltype(i)::value>(st, wave); });
-        static_for<NPB>([&](auto i) { ob.template issue_piece<decltype(i)::value>(st + RING_OPERAND_BYTES, wave); });
-        oa.advance(lda);
-        ob.advance(ldb);
-      }
-    }
-  }
-  // tile 0 must have landed for every wave before anyone reads it (the tiles behind it may be in flight)
-  static_assert((AHEAD - 1) * (NPA + NPB) + STORES < 64, "the counter's range");
-  if (STORES > 0 && stores && nk > AHEAD - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((AHEAD - 1) * (NPA + NPB) + STORES) : "memory");
-  else if (nk > AHEAD - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((AHEAD - 1) * (NPA + NPB)) : "memory");
-  else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-
-  u16x8 fa[2][MI], fb[2][NI];
-  // Read unit U of a half step: the B fragments first, then the A fragments.
-  auto read_unit = [&](auto unit_tag, auto s_tag, const SBAMD_LDS unsigned char* st, u16x8 (&xa)[MI], u16x8 (&xb)[NI]) {
-    constexpr int U = decltype(unit_tag)::value, S = decltype(s_tag)::value;
-    if constexpr (U < NI) xb[U] = OpB::template fragment<S>(st + RING_OPERAND_BYTES, wn * WTN + U * 32, lane);
-    else xa[U - NI] = OpA::template fragment<S>(st, wm * WTM + (U - NI) * 32, lane);
-  };
-  using yes = std::integral_constant<bool, true>;
-  using no = std::integral_constant<bool, false>;
-
-  // One half step with its issue order written out: matrix instruction n, then read
-  // unit n of the NEXT half step (six units for eight matrix instructions), a load
-  // piece behind the third and the sixth.  sched_barrier(0) keeps the compiler from
-  // regrouping; the operands of the matrix instructions were waited for before the
-  // last barrier, so nothing in here stalls on memory.
-  auto half_step = [&](auto s_next_tag, auto loads_tag, auto reads_tag, auto piece_tag, const SBAMD_LDS unsigned char* st_next,
-                       SBAMD_LDS unsigned char* fill, u16x8 (&ca)[MI], u16x8 (&cb)[NI], u16x8 (&na)[MI], u16x8 (&nb)[NI]) {
-    constexpr bool LOADS = decltype(loads_tag)::value, READS = decltype(reads_tag)::value;
-    constexpr int PIECE = decltype(piece_tag)::value;
-    auto slot = [&](auto n_tag) {
-      constexpr int N = decltype(n_tag)::value;
-      constexpr int I = N / NI, J = N % NI;
-      if constexpr (!(ABLATE & 2)) acc[I][J] = M_FIRST ? Mfma16<Tag>::mma(cb[J], ca[I], acc[I][J]) : Mfma16<Tag>::mma(ca[I], cb[J], acc[I][J]);
-      __builtin_amdgcn_sched_barrier(0);
-      if constexpr (READS && N < MI + NI && !(ABLATE & 4)) read_unit(std::integral_constant<int, N>{}, s_next_tag, st_next, na, nb);
-      if constexpr (LOADS && !(ABLATE & 1)) {
-        // this half step's load instructions (A's pieces, then B's) behind matrix instructions 2 and 5 of
-        // eight, 1 and 3 of four, 2 / 6 / 10 / 14 of sixteen
-        static_for<LPH>([&](auto l_tag) {
-          constexpr int L = decltype(l_tag)::value;
-          constexpr int AT = LPH == 2 ? (L == 0 ? NM / 4 : NM / 2 + NM / 4 - (NM > 4 ? 1 : 0)) : (2 * L + 1) * NM / (2 * LPH);
-          if constexpr (N == AT) {
-            if constexpr (L < LPA) oa.template issue_piece<PIECE * LPA + L>(fill, wave);
-            else ob.template issue_piece<PIECE * (LPH - LPA) + L - LPA>(fill + RING_OPERAND_BYTES, wave);
-          }
-        });
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    };
-    static_for<NM>(slot);
-  };
-  static_assert((NM == 16 || NM == 8 || NM == 4) && MI + NI <= NM, "wave tiles of 128 x 128, 128 x 64 and 64 x 64");
-
-  // first fragments of tile 0
-  {
-    static_for<MI + NI>([&](auto u) { read_unit(u, std::integral_constant<int, 0>{}, smem, fa[0], fb[0]); });
-  }
-
-  // One K step.  LOADS: tile t + AHEAD exists and is issued here; NEXT: tile
-  // t + 1 exists.
-  auto step = [&](const SBAMD_LDS unsigned char* cur, const SBAMD_LDS unsigned char* next, SBAMD_LDS unsigned char* fill,
-                  auto loads_tag, auto next_tag, auto extra_tag) {
-    constexpr bool LOADS = decltype(loads_tag)::value;
-    constexpr int EXTRA = decltype(extra_tag)::value;  // stores that may still be out as well
-
-    // the fragments fetched during the previous half step must have arrived (the
-    // transposing reads are inline assembly: the compiler does not wait for them)
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-
-    // first half step: matrix work on k 0..15, fragments of k 16..31, piece 0 of A and B
-    half_step(std::integral_constant<int, 1>{}, loads_tag, yes{}, std::integral_constant<int, 0>{}, cur, fill, fa[0], fb[0],
-              fa[1], fb[1]);
-
-    // every fragment read of tile t has returned; own pieces of tile t + 1 have landed
-    // (in flight and allowed to stay so: tiles t + 2 .. t + AHEAD - 1 and the first half of tile t + AHEAD)
-    if (LOADS && !(ABLATE & 1)) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((AHEAD - 2) * (NPA + NPB) + LPH + EXTRA) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-
-    // second half step: matrix work on k 16..31, first fragments of tile t + 1, piece 1
-    half_step(std::integral_constant<int, 0>{}, loads_tag, next_tag, std::integral_constant<int, 1>{}, next, fill, fa[1],
-              fb[1], fa[0], fb[0]);
-    if (LOADS) {
-      oa.advance(lda);
-      ob.advance(ldb);
-    }
-  };
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the first fragments
-  __builtin_amdgcn_sched_barrier(0);
-
-  // Steady state: as many steps per trip as there are stages, so that every LDS address is the lane's offset plus a
-  // compile-time constant.
-  int t = 0;
-  using none = std::integral_constant<int, 0>;
-  if constexpr (STORES > 0) {
-    // the tiles that were in flight before the stores: AHEAD - 1 of them are waited for in steps 0 .. AHEAD - 2
-    if (stores && t + STAGES - 1 + AHEAD < nk) {
-      static_for<STAGES>([&](auto i_tag) {
-        constexpr int I = decltype(i_tag)::value;
-        step(smem + I * RING_STAGE_BYTES, smem + (I + 1) % STAGES * RING_STAGE_BYTES, smem + (I + STAGES - 1) % STAGES * RING_STAGE_BYTES,
-             yes{}, yes{}, std::integral_constant<int, (I < AHEAD - 1 ? STORES : 0)>{});
-      });
-      t = STAGES;
-    }
-  }
-  for (; t + STAGES - 1 + AHEAD < nk; t += STAGES) {
-    static_for<STAGES>([&](auto i_tag) {
-      constexpr int I = decltype(i_tag)::value;
-      step(smem + I * RING_STAGE_BYTES, smem + (I + 1) % STAGES * RING_STAGE_BYTES, smem + (I + STAGES - 1) % STAGES * RING_STAGE_BYTES, yes{},
-           yes{}, none{});
-    });
-  }
-  // the remaining steps (t is a multiple of STAGES here) with the stage computed at run time
-  for (; t + AHEAD < nk; ++t) step(stage_ptr(t), stage_ptr(t + 1), stage_ptr(t + AHEAD), yes{}, yes{}, none{});
-  for (; t + 1 < nk; ++t) step(stage_ptr(t), stage_ptr(t + 1), stage_ptr(t + AHEAD), no{}, yes{}, none{});
-  if (t < nk) step(stage_ptr(t), stage_ptr(t + 1), stage_ptr(t + AHEAD), no{}, no{}, none{});
-
-  // K tail (k % 32 valid k): one more tile, zero-padded, staged through registers into stage 0 once every
-  // wavefront has finished the last ring step; the zeros add nothing to the sums.
-  const int k_rem = int(k_len - int64_t(nk) * RING_BK);
-  if (k_rem > 0) {
-    __syncthreads();
-    u16x8 ta[NPA], tb[NPB];
-    static_for<NPA>([&](auto i) { ta[decltype(i)::value] = oa.template load_tail<decltype(i)::value>(k_rem, tid); });
-    static_for<NPB>([&](auto i) { tb[decltype(i)::value] = ob.template load_tail<decltype(i)::value>(k_rem, tid); });
-    static_for<NPA>([&](auto i) { OpA::template store_tail<decltype(i)::value>(smem, tid, ta[decltype(i)::value]); });
-    static_for<NPB>([&](auto i) { OpB::template store_tail<decltype(i)::value>(smem + RING_OPERAND_BYTES, tid, tb[decltype(i)::value]); });
-    __syncthreads();
-    auto tail_half = [&](auto s_tag) {
-      static_for<MI + NI>([&](auto u) { read_unit(u, s_tag, smem, fa[0], fb[0]); });
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the transposing reads are not tracked by the compiler
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int i = 0; i < MI; ++i)
-#pragma unroll
-        for (int j = 0; j < NI; ++j) acc[i][j] = M_FIRST ? Mfma16<Tag>::mma(fb[0][j], fa[0][i], acc[i][j]) : Mfma16<Tag>::mma(fa[0][i], fb[0][j], acc[i][j]);
-      __builtin_amdgcn_sched_barrier(0);
-    };
-    tail_half(std::integral_constant<int, 0>{});
-    if (k_rem > 16) tail_half(std::integral_constant<int, 1>{});
-  }
-}
-
-// The same first loads, for a caller that issues them ahead of other work.
-template <typename OpA, typename OpB, int STAGES>
+// The first RING_AHEAD tiles (those that exist) go in flight.
+template <typename OpA, typename OpB>
 __device__ __attribute__((always_inline)) inline void ring_start(OpA& oa, OpB& ob, const int64_t lda, const int64_t ldb, const int nk,
                                                                  SBAMD_LDS unsigned char* smem, const int wave) {
-  constexpr int NPA = OpA::NP, NPB = OpB::NP;
-  constexpr int AHEAD = STAGES - 1;
   constexpr int RING_OPERAND_BYTES = OpA::BYTES;
   constexpr int RING_STAGE_BYTES = OpA::BYTES + OpB::BYTES;
 #pragma unroll
-  for (int t = 0; t < AHEAD; ++t) {
+  for (int t = 0; t < RING_AHEAD; ++t) {
     if (t < nk) {
       SBAMD_LDS unsigned char* st = smem + t * RING_STAGE_BYTES;
-      static_for<NPA>([&](auto i) { oa.template issue_piece<decltype(i)::value>(st, wave); });
-      static_for<NPB>([&](auto i) { ob.template issue_piece<decltype(i)::value>(st + RING_OPERAND_BYTES, wave); });
+      static_for<OpA::NP>([&](auto i) { oa.template issue_piece<decltype(i)::value>(st, wave); });
+      static_for<OpB::NP>([&](auto i) { ob.template issue_piece<decltype(i)::value>(st + RING_OPERAND_BYTES, wave); });
       oa.advance(lda);
       ob.advance(ldb);
     }
   }
 }
 
+// The ring as a function (see gemm_half_ring.hpp for the names).
+template <typename Tag, typename OpA, typename OpB, int MI, int NI, int WTM, int WTN, int ABLATE, bool M_FIRST, int STORES, typename Acc>
+__device__ __attribute__((always_inline)) inline void ring_multiply(Acc (&acc)[MI][NI], OpA& oa, OpB& ob, const int64_t lda, const int64_t ldb,
+                                                                    const int64_t k_len, SBAMD_LDS unsigned char* smem, const int tid,
+                                                                    const int lane, const int wave, const int wm, const int wn, const bool stores) {
+#include "gemm_half_ring.hpp"
+}
+
+// ABLATE is a timing-only diagnostic (bit 1: no loads inside the K loop, bit 2: no matrix
+// instructions, bit 4: no fragment reads); the library instantiates 0.
 // BM x BN tile on WM x WN wavefronts: 256 x 256 on 2 x 4 (wave tile 128 x 64) or on 2 x 2 (wave tile 128 x 128: one
 // wavefront per SIMD with 256 accumulator registers, a third fewer fragment bytes per flop), 128 x 128 on 2 x 2 (64 x 64).
 template <typename Tag, typename TOut, bool TA, bool TB, int ABLATE = 0, int BM = DMA_BM, int BN = DMA_BN, int WM = 2, int WN = 4>
@@ -454,7 +286,11 @@ __global__ void __launch_bounds__(WM* WN * 64, ((BM / WM) * (BN / WN) > 128 * 64
   OpB ob;
   oa.init(a, g.lda, m0, g.lim_a > 0 ? g.lim_a : g.m, tid);
   ob.init(b, g.ldb, n0, g.lim_b > 0 ? g.lim_b : g.n, tid);
-  ring_multiply<Tag, OpA, OpB, MI, NI, WTM, WTN, ABLATE, true, RING_STAGES, false>(acc, oa, ob, g.lda, g.ldb, k_len, smem, tid, lane, wave, wm, wn);
+  ring_start(oa, ob, g.lda, g.ldb, int(k_len / RING_BK), smem, wave);
+  constexpr bool M_FIRST = true, stores = false;
+  constexpr int STORES = 0;
+  const int64_t lda = g.lda, ldb = g.ldb;
+#include "gemm_half_ring.hpp"
 
   const int frag_mn = lane & 31, frag_h = lane >> 5;
   auto value = [&](int i, int j, int r) -> float { return g.alpha * acc[i][j][r]; };
