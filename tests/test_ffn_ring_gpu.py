@@ -135,7 +135,7 @@ def test_whole_and_cut_tiles_in_one_launch(h, out, beta, n, m, k):
 
 # ------------------------------------------------------------------- gradient
 def exact_grad(h, dtype, n, m, k, ta="t", tb="n", pad=0, shift=0, beta_a=0.0, beta_b=0.0, want="ab", family=RING256, top=2, check_cut=None,
-               repeat=1):
+               repeat=1, in_place=False):
     """ReLU and whole numbers: dP is exact, and so are the sums behind dA and dB."""
     rng = seeded("exact gradient", dtype, n, m, k, ta, tb, pad, shift, beta_a, beta_b, want)
     x, w, p, dh = (whole(rng, top, *s) for s in ((n, k), (2 * m, k), (n, 2 * m), (n, m)))
@@ -151,6 +151,7 @@ def exact_grad(h, dtype, n, m, k, ta="t", tb="n", pad=0, shift=0, beta_a=0.0, be
     wg, xg = weights(w), tokens(x)
     pg = Mat(h, dtype, n, 2 * m, 2 * m + pad, shift, bits(p, dtype))
     dcg, dpg = Mat(h, dtype, n, m, m + pad, shift, bits(dh, dtype)), Mat(h, dtype, n, 2 * m, 2 * m + pad, shift)
+    dpg = pg if in_place else dpg
     h.set_kernel(*family)
     for _ in range(repeat):
         dag, dbg = weights(da0) if "a" in want else None, tokens(db0) if "b" in want else None
@@ -185,6 +186,15 @@ def test_grad_whole_and_cut_tiles_in_one_launch(h, dtype, ta, tb):
     n, m, k = 2208, 2176, 4096
     exact_grad(h, dtype, n, m, k, ta, tb, want="a", top=1, check_cut=True)
     exact_grad(h, dtype, n, m, k, ta, tb, top=1, repeat=2)
+
+
+@pytest.mark.parametrize("family", FAMILIES)
+@pytest.mark.parametrize("ta,tb", [("t", "n"), ("n", "t")])
+@pytest.mark.parametrize("n,m,k,pad", [(1104, 302, 136, 0), (77, 29, 40, 0), (520, 130, 64, 6)])
+def test_grad_in_place_of_p(h, family, n, m, k, pad, ta, tb):
+    """dP over P where the products read a padded copy of it (2m and its rows no multiple of 8) and where they do not."""
+    exact_grad(h, "bfloat16", n, m, k, ta, tb, pad=pad, family=FAMILIES[family], in_place=True)
+    exact_grad(h, "float16", n, m, k, ta, tb, pad=pad, family=FAMILIES[family], in_place=True, want="b")
 
 
 def test_grad_tiles_in_turn(h):
