@@ -14,8 +14,9 @@
  * operand in the handle's own scratch area.
  *
  * Scratch and graphs: repacked operands and products cut along k use scratch areas of the handle, which grow
- * at the first call that needs them; such a call has to have run once before it is captured, and graphs captured
- * from one handle share the areas, so they must not replay at the same time.
+ * at the first call that needs them; such a call has to have run once before it is captured.  Graphs captured
+ * from one handle and the handle's ordinary calls share the areas: on the handle's own stream they run one after the
+ * other, but a replay on another stream must not run beside another such replay or beside calls of the handle.
  *
  * sbamd_set_kernel pins SBAMD_KERNEL_SMALL (few tokens), _LARGE (128 x 128 tiles) or _HUGE (256 x 256);
  * sbamd_last_kernel and sbamd_last_splitk report what ran; after a gradient, its last product (-1 if it had none).

@@ -88,8 +88,8 @@ struct FfnArgs {
 };
 
 // ---------------------------------------------------------------- activations
-// e^x through the hardware's 2^x (1 ulp): the argument's rounding makes it good to about |x| * 2^-24, far below
-// the 16-bit roundings behind it and within 4e-6 for a float result.  Overflow gives infinity and a quotient of 0.
+// e^x through the hardware's 2^x (1 ulp): the roundings of the argument and of log2(e) make it good to about |x| * 2^-23.6, far
+// below the 16-bit roundings behind it and within 7e-6 for a float result.  Overflow gives infinity and a quotient of 0.
 __device__ inline float ffn_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
 __device__ inline float ffn_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + ffn_exp(-x)); }
 
@@ -97,8 +97,9 @@ __device__ inline float ffn_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f
 __device__ inline float gelu_tanh_arg2(float g) { return 1.5957691216057308f * (g + 0.044715f * g * g * g); }
 
 // Phi(g) and e^(-g^2/2), one exponential for both: with x = |g| / sqrt(2), erfc(x) = e^(-x^2) R(x), and R is a polynomial in
-// t = 1 / (1 + 0.4 x), fitted for the least largest relative error over 0 <= x <= 9.5 (8.4e-8; 4.3e-7 as evaluated in float), so the
-// small values of Phi far on the negative side keep their relative precision, which 1 + erf would cancel away.
+// t = 1 / (1 + 0.4 x), fitted for the least largest relative error over 0 <= x <= 9.5 (1.6e-7 with the coefficients as stored,
+// below 5e-7 as evaluated in float), so the small values of Phi far on the negative side keep their relative
+// precision, which 1 + erf would cancel away.
 // (With the device library's erfc the elementwise gradient took 11.8 us at 1119 x 2730, so 8.5.)
 __device__ inline void normal_parts(float g, float& phi, float& bell) {
   const float x = __builtin_fabsf(g) * 0.70710678118654752f;
@@ -940,7 +941,10 @@ __global__ void __launch_bounds__(TPC < 256 ? 256 : TPC)
 
 // -------------------------------------------------- gradient, elementwise half
 // dG = dC U act'(G), dU = dC act(G): eight channels of one token per thread.  p and dp may be the same matrix: a thread
-// reads what it overwrites, and nothing else, before it writes.  (Hence no __restrict__ on them.)  copy: NULL, or a second
+// reads what it overwrites, and nothing else, before it writes.  (Hence no __restrict__ on them.)
+// dP is rounded to the storage type because the products' matrix instructions take 16-bit operands (a second, low half of it
+// would double their time): dA and dB carry sqrt(2) of one rounding's error (relative to 64 bits, half 2.9e-4 where one
+// rounding makes 2.1e-4, bfloat16 2.4e-3 and 1.7e-3).  copy: NULL, or a second
 // dP with aligned rows of ld_copy (a multiple of 8) elements, zeros behind 2m, for products that need whole 16-byte pieces.
 template <typename Tag, typename TOut>
 __global__ void __launch_bounds__(256)

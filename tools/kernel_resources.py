@@ -6,6 +6,7 @@ import subprocess
 import sys
 
 out = subprocess.run(["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "--offload-arch=gfx950", "-ffp-contract=off",
+                      "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",  # as the library is built
                       "-Rpass-analysis=kernel-resource-usage", "-c", sys.argv[1], "-o", "/dev/null"],
                      capture_output=True, text=True).stderr
 flt = sys.argv[2] if len(sys.argv) > 2 else ""
